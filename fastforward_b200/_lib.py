@@ -15,6 +15,7 @@ OK, EINVAL, EUNSUPPORTED, ECUDA, ETIMEOUT = 0, -1, -2, -3, -4
 QUANT_NONE, QUANT_STATIC, QUANT_ROWWISE, QUANT_ROWSCALE = 0, 1, 2, 3
 EPI_BF16, EPI_F32_PARTIAL, EPI_SWIGLU = 0, 1, 2
 EPI_BIAS, EPI_BIAS_RES, EPI_BIAS_GELU_TANH, EPI_BIAS_GELU_ERF = 10, 11, 12, 13  # ffb_bf16_gemm
+KV4_PAGE, KV4_RECORD = 64, 9216  # tokens of a page; bytes of one page of one K/V head
 TILE_STREAM = 1  # ffb_fp8_gemm feature_tile: the weight-stationary schedule
 PRO_QUANT, PRO_ADD_RMSNORM = 1, 2
 
@@ -80,7 +81,15 @@ SIGNATURES = {
     "ffb_add_layernorm": [P, P, P, P, F, P, P, I, I, P],
     "ffb_vision_rope": [P, P, P, I, I, I, I, P, P, P, P],
     "ffb_attention_full": [P, P, P, P, I, I, I, F, P],
+    "ffb_qk_norm_rope_kv4": [P, c_int64, P, P, F, P, P, P, P, I, P, c_int64, I, P, P, I, I, I, I, P],
+    "ffb_kv4_read": [P, I, P, c_int64, I, P, P, P, P, I, I, I, P],
+    "ffb_attention_kv4": [P, P, I, P, c_int64, I, P, P, P, P, c_int64, I, I, I, I, I, F, I, I, P],
+    "ffb_attention_kv4_workspace": [I, I, I, I, I, I, I, I],
 }
+
+
+# return types other than an int status
+_RESTYPES = {"ffb_version": c_char_p, "ffb_attention_kv4_workspace": c_int64}
 
 
 class FFBError(RuntimeError):
@@ -104,7 +113,7 @@ def lib():
         for name, args in SIGNATURES.items():
             fn = getattr(handle, name)
             fn.argtypes = args
-            fn.restype = c_char_p if name == "ffb_version" else c_int
+            fn.restype = _RESTYPES.get(name, c_int)
         _lib = handle
     return _lib
 

@@ -1,0 +1,580 @@
+// Attention over the 4-bit paged K/V cache (layout: kv4.cuh) for few query rows a sequence:
+// single-token decoding and short runs of new tokens.
+//
+//   o[t, h] = sum_j p_j v_j / sum_j p_j,  p_j = 2^(x_j - m),  x_j = scale log2(e) q.k_j
+// over the keys j <= the row's position, inside the window or among the first `sinks`.
+//
+// The floor is the bytes of the visible pages (144 a token and K/V head), so the kernel is
+// built to keep bulk copies in flight and to spend few instructions a byte:
+//   - one CTA takes one (sequence, K/V head, 8 NT query columns, share of the pages): the
+//     columns are the (row, head of the group) pairs, so a page is read once for all the
+//     query heads that share it.  16 warps in four groups; a group has its own ring of
+//     STAGES page records, filled by cp.async.bulk, and its four warps take 16 tokens each;
+//   - the products run on mma.sync m16n8k16 with the tokens on M and the query columns on N
+//     (S^T = K Q^T, O^T = V^T P^T): with G <= 8 heads a group a tcgen05 tile of 128 rows
+//     would be nearly empty, and its operands would have to be written to shared memory as
+//     bf16, four times the bytes of the codes.  Here a code becomes bf16 in a register:
+//     0x4300 | nibble is 128 + nibble;
+//   - K: the offset 136 of every operand is taken out by starting each group's accumulator at
+//     -136 sum(q) of the group's channels; the group's scale multiplies the fp32 sums;
+//   - V: the offset is subtracted (exact), the scale multiplies the probability before its
+//     one rounding to bf16, once per group of channels; P^T is formed by movmatrix;
+//   - the running maximum moves only when a score passes it by more than 8 (in base 2), which
+//     a vote finds: p <= 2^8, nothing overflows, and the rescaling is rare.
+// S, the maxima, the sums and O are fp32; P (times V's scale) is rounded to bf16, the type of
+// the tensor core's operand, with relative error 2^-9 of each term.
+// Shares of a long axis are joined by kv4_combine_kernel (fp32 partials in the workspace).
+#include "kv4.cuh"
+#include "pdl.cuh"
+
+#include <math.h>
+#include <type_traits>
+
+namespace {
+
+using namespace kv4;
+
+constexpr int GROUPS = 4;             // page streams of a CTA
+constexpr int THREADS = GROUPS * 128;
+constexpr int STAGES = 5;             // page records in flight per group
+constexpr int RING = GROUPS * STAGES * RECORD;
+constexpr int CS = D + 4;             // fp32 pitch of a column in the final exchange (spreads the banks)
+constexpr int BAR_BYTES = 2 * GROUPS * STAGES * 8 + GROUPS * STAGES * 4 + 16;
+constexpr float LAZY = 8.f;
+
+template <int NT>
+constexpr int smem_bytes() {  // ring | Q fragments [NT][4][32] uint4 | offsets [NT][2][32] float4 | barriers
+  return RING + NT * 4 * 512 + NT * 2 * 512 + BAR_BYTES + 128;
+}
+
+struct Args {
+  const uint16_t* q;  // [HQ, T, 128]
+  uint16_t* out;      // [T, HQ, 128]
+  float* part_o;      // [splits][T * HQ][128], relative to part_ml's maximum (splits > 1)
+  float* part_ml;     // [splits][T * HQ][2]
+  Seqs seqs;
+  int HQ, splits, window, sinks;
+  float scale_log2;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+// Nibbles i and i + 4 of w as the bf16 pair (136 + code).
+__device__ __forceinline__ uint32_t pair136(uint32_t w, int i) { return ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u; }
+__device__ __forceinline__ uint32_t minus136(uint32_t w) {
+  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&w), __floats2bfloat162_rn(136.f, 136.f));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float lo_of(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float hi_of(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+// The token of fragment row r (0..7): 2 <-> 3 and 6 <-> 7 trade places, so that the eight lanes
+// of a load phase meet rows of both parities and, with V's exchanged halves, all banks.
+__device__ __forceinline__ int token_of(int r) { return r ^ ((r >> 1) & 1); }
+
+// The pages that a tile of rows [first, last] (positions) reads: the first n_sink pages, then
+// [first_page, first_page + n - n_sink).
+struct PageSet {
+  int n, n_sink, first_page, first_key, kend;
+};
+__device__ __forceinline__ PageSet pages_of(int pos_lo, int pos_hi, int max_pages, int window, int sinks) {
+  PageSet s;
+  s.kend = min(pos_hi + 1, max_pages * PAGE);
+  s.first_key = window > 0 ? max(0, pos_lo - window + 1) : 0;
+  s.first_page = s.first_key / PAGE;
+  s.n_sink = window > 0 ? min((min(sinks, max(s.kend, 0)) + PAGE - 1) / PAGE, s.first_page) : 0;
+  s.n = s.kend > 0 ? s.n_sink + max(0, (s.kend + PAGE - 1) / PAGE - s.first_page) : 0;
+  return s;
+}
+
+template <int NT>
+__global__ void __launch_bounds__(THREADS, 1) kv4_attention_kernel(const Args args) {
+  constexpr int QT = 8 * NT;
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
+  uint4* sq = reinterpret_cast<uint4*>(smem + RING);                     // [NT][4][32]
+  float4* soff = reinterpret_cast<float4*>(smem + RING + NT * 4 * 512);  // [NT][2][32]
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + RING + NT * 6 * 512);
+  uint64_t* empty = full + GROUPS * STAGES;
+  int* bad = reinterpret_cast<int*>(empty + GROUPS * STAGES);  // per stage: the page id was outside the cache
+  volatile int* abort_flag = bad + GROUPS * STAGES;
+
+  const Seqs& sq_ = args.seqs;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int group = warp >> 2, w4 = warp & 3, g = lane >> 2, t = lane & 3;
+  const int split = blockIdx.x % args.splits;
+  const int kvh = (blockIdx.x / args.splits) % sq_.HK, b = blockIdx.x / (args.splits * sq_.HK);
+  const int G = args.HQ / sq_.HK;
+
+  if (tid == 0) {
+    for (int i = 0; i < GROUPS * STAGES; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 4);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  pdl_wait();
+  if (tid == 0) pdl_launch();
+
+  const int r0 = min(max(__ldg(sq_.row_start + b), 0), sq_.T);
+  const int r1 = min(max(__ldg(sq_.row_start + b + 1), r0), sq_.T);
+  const int S = r1 - r0, ctx = max(__ldg(sq_.ctx_len + b), 0);
+  const int ncols = S * G;
+  const int* table = sq_.table + b * sq_.table_stride;
+  uint32_t used = 0;  // stages this group has used so far (over all query tiles)
+  if (ctx > sq_.max_pages * PAGE && S > 0 && tid == 0) atomicOr(&ffb_device_error_word, (uint32_t)ffb::ERR_KV4_PAGE);
+
+  for (int c0 = (int)blockIdx.y * QT; c0 < ncols; c0 += (int)gridDim.y * QT) {
+    const int clast = min(c0 + QT, ncols) - 1;
+    const int pos_lo = ctx - S + c0 / G, pos_hi = ctx - S + clast / G;
+    const PageSet ps = pages_of(pos_lo, pos_hi, sq_.max_pages, args.window, args.sinks);
+    const int i0 = (int)((int64_t)split * ps.n / args.splits), i1 = (int)((int64_t)(split + 1) * ps.n / args.splits);
+    const int cnt = max(0, (i1 - i0 - group + GROUPS - 1) / GROUPS);  // pages i0 + group + GROUPS k of this group
+    auto page_index = [&](int k) {
+      const int i = i0 + group + GROUPS * k;
+      return i < ps.n_sink ? i : ps.first_page + i - ps.n_sink;
+    };
+    auto issue = [&](int k) {  // one lane
+      const uint32_t u = used + k;
+      const int s = group * STAGES + u % STAGES;
+      const int page = __ldg(table + page_index(k));
+      const bool ok = page >= 0 && page < sq_.num_pages;
+      bad[s] = !ok;
+      if (ok) {
+        mbar_arrive_expect_tx(&full[s], RECORD);
+        bulk_load(smem + s * RECORD, sq_.pages + ((int64_t)page * sq_.HK + kvh) * RECORD, RECORD, &full[s]);
+      } else {
+        atomicOr(&ffb_device_error_word, (uint32_t)ffb::ERR_KV4_PAGE);
+        mbar_arrive(&full[s]);
+      }
+    };
+    int issued = 0;
+    if (w4 == 0 && lane == 0)
+      for (; issued < min(cnt, STAGES); ++issued) issue(issued);
+
+    // query fragments of this tile, once per CTA: lane (g, t) of column tile n holds channels
+    // 32 j + 8 t .. + 7 of column 8 n + g as the pairs (e, e + 4) that pair136 gives
+    for (int f = warp; f < 4 * NT; f += THREADS / 32) {
+      const int n = f >> 2, j = f & 3;
+      const int c = c0 + 8 * n + g;
+      uint4 x = make_uint4(0u, 0u, 0u, 0u);
+      if (c <= clast) {
+        const int row = r0 + c / G, h = kvh * G + c % G;
+        x = __ldg(reinterpret_cast<const uint4*>(args.q + ((int64_t)h * sq_.T + row) * D + 32 * j + 8 * t));
+      }
+      float sum = lo_of(x.x) + hi_of(x.x) + lo_of(x.y) + hi_of(x.y) + lo_of(x.z) + hi_of(x.z) + lo_of(x.w) + hi_of(x.w);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      sq[(n * 4 + j) * 32 + lane] = make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632),
+                                               __byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632));
+      // lane (g', t') of the score fragment needs the sums of columns 2 t' and 2 t' + 1
+      const float s0 = __shfl_sync(0xffffffffu, sum, 8 * t), s1 = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+      float2* dst = reinterpret_cast<float2*>(soff) + ((n * 2 + (j >> 1)) * 32 + lane) * 2 + (j & 1);
+      *dst = make_float2(-136.f * s0, -136.f * s1);
+    }
+    __syncthreads();
+
+    uint32_t qf[NT == 1 ? 16 : 1];
+    float off[NT == 1 ? 8 : 1];
+    if constexpr (NT == 1) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint4 x = sq[j * 32 + lane];
+        qf[4 * j] = x.x; qf[4 * j + 1] = x.y; qf[4 * j + 2] = x.z; qf[4 * j + 3] = x.w;
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float4 x = soff[j * 32 + lane];
+        off[4 * j] = x.x; off[4 * j + 1] = x.y; off[4 * j + 2] = x.z; off[4 * j + 3] = x.w;
+      }
+    }
+
+    float o[8][NT][4], m[2 * NT], l[2 * NT];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][n][e] = 0.f;
+    int pos[2 * NT];  // positions of this lane's columns
+#pragma unroll
+    for (int i = 0; i < 2 * NT; ++i) {
+      m[i] = -INFINITY;
+      l[i] = 0.f;
+      const int c = c0 + 8 * (i >> 1) + 2 * t + (i & 1);
+      pos[i] = c <= clast ? ctx - S + c / G : -1;
+    }
+
+    // sixteen tokens of one page; MASKED: some column may not see some of them
+    auto tile = [&](const uint8_t* rec, int key0, auto masked_tag) {
+      constexpr bool MASKED = decltype(masked_tag)::value;
+      const int ra = 16 * w4 + token_of(g), rb = ra + 8;  // tokens of fragment rows g and g + 8
+      float s[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+      {
+        const uint4 ka = *reinterpret_cast<const uint4*>(rec + 64 * ra + 16 * t);
+        const uint4 kb = *reinterpret_cast<const uint4*>(rec + 64 * rb + 16 * t);
+        const uint2 sa = *reinterpret_cast<const uint2*>(rec + K_SCALES + 8 * ra);
+        const uint2 sb = *reinterpret_cast<const uint2*>(rec + K_SCALES + 8 * rb);
+        const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+        const float fa[4] = {lo_of(sa.x), hi_of(sa.x), lo_of(sa.y), hi_of(sa.y)};
+        const float fb[4] = {lo_of(sb.x), hi_of(sb.x), lo_of(sb.y), hi_of(sb.y)};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t a0 = pair136(wa[j], 0), a1 = pair136(wb[j], 0), a2 = pair136(wa[j], 1), a3 = pair136(wb[j], 1);
+          const uint32_t a4 = pair136(wa[j], 2), a5 = pair136(wb[j], 2), a6 = pair136(wa[j], 3), a7 = pair136(wb[j], 3);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            uint32_t q0, q1, q2, q3;
+            float c[4];
+            if constexpr (NT == 1) {
+              q0 = qf[4 * j]; q1 = qf[4 * j + 1]; q2 = qf[4 * j + 2]; q3 = qf[4 * j + 3];
+              c[0] = off[2 * j]; c[1] = off[2 * j + 1];
+            } else {
+              const uint4 x = sq[(n * 4 + j) * 32 + lane];
+              q0 = x.x; q1 = x.y; q2 = x.z; q3 = x.w;
+              const float2 y = reinterpret_cast<const float2*>(soff)[((n * 2 + (j >> 1)) * 32 + lane) * 2 + (j & 1)];
+              c[0] = y.x; c[1] = y.y;
+            }
+            c[2] = c[0];
+            c[3] = c[1];
+            mma16816(c, a0, a1, a2, a3, q0, q1);
+            mma16816(c, a4, a5, a6, a7, q2, q3);
+            s[n][0] = fmaf(c[0], fa[j], s[n][0]);
+            s[n][1] = fmaf(c[1], fa[j], s[n][1]);
+            s[n][2] = fmaf(c[2], fb[j], s[n][2]);
+            s[n][3] = fmaf(c[3], fb[j], s[n][3]);
+          }
+        }
+      }
+      bool grow = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float x = s[n][e] * args.scale_log2;
+          if constexpr (MASKED) {
+            const int key = key0 + (e < 2 ? ra : rb), p = pos[2 * n + (e & 1)];
+            if (key > p || key >= ps.kend || (args.window > 0 && p - key >= args.window && key >= args.sinks)) x = -INFINITY;
+          }
+          s[n][e] = x;
+          grow |= x > m[2 * n + (e & 1)] + LAZY;
+        }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int i = 0; i < 2 * NT; ++i) {
+          float x = fmaxf(s[i >> 1][i & 1], s[i >> 1][2 + (i & 1)]);
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+          const float nm = fmaxf(m[i], x);
+          const float a = nm == -INFINITY ? 1.f : ex2(m[i] - nm);  // nothing seen yet: keep zeros
+          m[i] = nm;
+          l[i] *= a;
+#pragma unroll
+          for (int d = 0; d < 8; ++d) {
+            o[d][i >> 1][i & 1] *= a;
+            o[d][i >> 1][2 + (i & 1)] *= a;
+          }
+        }
+      }
+      uint32_t pb[NT][8];  // P^T fragments, V's scale of group j folded in
+      {
+        const uint2 sa = *reinterpret_cast<const uint2*>(rec + V_SCALES + 8 * ra);
+        const uint2 sb = *reinterpret_cast<const uint2*>(rec + V_SCALES + 8 * rb);
+        const float fa[4] = {lo_of(sa.x), hi_of(sa.x), lo_of(sa.y), hi_of(sa.y)};
+        const float fb[4] = {lo_of(sb.x), hi_of(sb.x), lo_of(sb.y), hi_of(sb.y)};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float p[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            // a masked score stays 0 even while the maximum is still -inf
+            p[e] = MASKED && s[n][e] == -INFINITY ? 0.f : ex2(s[n][e] - m[2 * n + (e & 1)]);
+            l[2 * n + (e & 1)] += p[e];
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float y[4] = {p[0] * fa[j], p[1] * fa[j], p[2] * fb[j], p[3] * fb[j]};
+            if constexpr (MASKED) {  // nothing of a masked token counts, whatever its scale holds
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (p[e] == 0.f) y[e] = 0.f;
+            }
+            pb[n][2 * j] = transpose8x8(pack_bf16(y[0], y[1]));
+            pb[n][2 * j + 1] = transpose8x8(pack_bf16(y[2], y[3]));
+          }
+        }
+      }
+      // V^T fragments: columns 2t, 2t+1, 2t+8, 2t+9 of the MMA are these four tokens
+      const int ta = 16 * w4 + token_of(2 * t), tb = 16 * w4 + token_of(2 * t + 1);
+      const uint8_t* v = rec + V_CODES + 8 * (g ^ (4 * (t >> 1)));
+      const uint2 v0 = *reinterpret_cast<const uint2*>(v + 64 * ta), v1 = *reinterpret_cast<const uint2*>(v + 64 * tb);
+      const uint2 v2 = *reinterpret_cast<const uint2*>(v + 64 * ta + 512), v3 = *reinterpret_cast<const uint2*>(v + 64 * tb + 512);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t x0 = half ? v0.y : v0.x, x1 = half ? v1.y : v1.x, x2 = half ? v2.y : v2.x, x3 = half ? v3.y : v3.x;
+#pragma unroll
+        for (int quart = 0; quart < 2; ++quart) {
+          const uint32_t sel = quart ? 0x7632 : 0x5410;
+          const uint32_t lo = __byte_perm(x0, x1, sel), hi = __byte_perm(x2, x3, sel);  // tokens (2t, 2t+1), (2t+8, 2t+9)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int mt = 4 * half + 2 * quart + u;  // channels 16 mt + g and 16 mt + 8 + g
+            const uint32_t a0 = minus136(pair136(lo, 2 * u)), a1 = minus136(pair136(lo, 2 * u + 1));
+            const uint32_t a2 = minus136(pair136(hi, 2 * u)), a3 = minus136(pair136(hi, 2 * u + 1));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma16816(o[mt][n], a0, a1, a2, a3, pb[n][2 * (mt >> 1)], pb[n][2 * (mt >> 1) + 1]);
+          }
+        }
+      }
+    };
+
+    bool ok = true;
+    for (int k = 0; k < cnt; ++k) {
+      const uint32_t u = used + k;
+      const int s = group * STAGES + u % STAGES;
+      // one verdict for the warp: its lanes stay together whatever each of them saw
+      if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full[s], (u / STAGES) & 1u, abort_flag))) {
+        ok = false;
+        break;
+      }
+      const int key0 = page_index(k) * PAGE;
+      if (!bad[s] && key0 + 16 * w4 < ps.kend) {
+        const uint8_t* rec = smem + s * RECORD;
+        const bool whole = key0 + PAGE - 1 <= pos_lo && key0 + PAGE <= ps.kend &&
+                           (args.window == 0 || pos_hi - key0 < args.window || key0 + PAGE <= args.sinks);
+        if (whole) tile(rec, key0, std::integral_constant<bool, false>{});
+        else tile(rec, key0, std::integral_constant<bool, true>{});
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[s]);
+      // refill the stage of the page before this one (its four warps are about to be done)
+      if (w4 == 0 && lane == 0 && k > 0 && issued < cnt) {
+        const uint32_t f = used + k - 1;
+        if (mbar_wait_bounded(&empty[group * STAGES + f % STAGES], (f / STAGES) & 1u, abort_flag)) issue(issued++);
+        else *abort_flag = 1;  // the waits for the pages never issued give up on it
+      }
+    }
+    // every stage of this tile is waited for before the ring is used again: `used` counts
+    // whole tiles, and the stages not waited on as empty above are drained here
+    if (!ok) *abort_flag = 1;
+    if (w4 == 0 && lane == 0) {
+      volatile int never = 0;
+      if (*abort_flag) {  // copies in flight must land before the CTA leaves
+        for (int k = max(0, issued - STAGES); k < issued; ++k)
+          mbar_wait_bounded(&full[group * STAGES + (used + k) % STAGES], ((used + k) / STAGES) & 1u, &never, 200000000ull);
+      } else {
+        for (int k = max(0, cnt - STAGES); k < cnt; ++k)
+          if (!mbar_wait_bounded(&empty[group * STAGES + (used + k) % STAGES], ((used + k) / STAGES) & 1u, abort_flag)) *abort_flag = 1;
+      }
+    }
+    used += cnt;
+#pragma unroll
+    for (int i = 0; i < 2 * NT; ++i) {
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 4);
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 8);
+      l[i] += __shfl_xor_sync(0xffffffffu, l[i], 16);
+    }
+    __syncthreads();  // all pages consumed: the ring becomes the exchange buffer
+    if (*abort_flag) break;  // uniform: read after the barrier that follows every write
+    // [16 warps][QT] maxima, sums, then [16 warps][QT][CS] outputs; NT = 2 in two rounds of 8 columns
+    float* xm = reinterpret_cast<float*>(smem);
+    float* xl = xm + 16 * QT;
+    float* xo = xl + 16 * QT;
+    if (g == 0) {
+#pragma unroll
+      for (int i = 0; i < 2 * NT; ++i) {
+        const int c = 8 * (i >> 1) + 2 * t + (i & 1);
+        xm[warp * QT + c] = m[i];
+        xl[warp * QT + c] = l[i];
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      if (n > 0) __syncthreads();
+#pragma unroll
+      for (int mt = 0; mt < 8; ++mt) {
+        float* dst = xo + (warp * 8 + 2 * t) * CS + 16 * mt + g;
+        dst[0] = o[mt][n][0];
+        dst[CS] = o[mt][n][1];
+        dst[8] = o[mt][n][2];
+        dst[CS + 8] = o[mt][n][3];
+      }
+      __syncthreads();
+      // 8 columns x 128 channels over 512 threads: two neighbouring channels a thread
+      const int c = tid >> 6, d = 2 * (tid & 63);
+      const int col = c0 + 8 * n + c;
+      if (col <= clast) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) top = fmaxf(top, xm[w * QT + 8 * n + c]);
+        float sum = 0.f, y0 = 0.f, y1 = 0.f;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) {
+          const float mw = xm[w * QT + 8 * n + c];
+          if (mw == -INFINITY && xl[w * QT + 8 * n + c] == 0.f) continue;  // this warp saw nothing of the row
+          const float f = ex2(mw - top);
+          const float2 v = *reinterpret_cast<const float2*>(xo + (w * 8 + c) * CS + d);
+          sum = fmaf(xl[w * QT + 8 * n + c], f, sum);
+          y0 = fmaf(v.x, f, y0);
+          y1 = fmaf(v.y, f, y1);
+        }
+        const int row = r0 + col / G, h = kvh * G + col % G;
+        const int64_t at = (int64_t)row * args.HQ + h;
+        if (args.splits == 1) {
+          const float r = sum == 0.f ? 0.f : 1.f / sum;  // nothing visible: zeros
+          *reinterpret_cast<uint32_t*>(args.out + at * D + d) = pack_bf16(y0 * r, y1 * r);
+        } else {
+          const int64_t pt = (int64_t)split * sq_.T * args.HQ + at;
+          *reinterpret_cast<float2*>(args.part_o + pt * D + d) = make_float2(y0, y1);
+          if (d == 0) *reinterpret_cast<float2*>(args.part_ml + pt * 2) = make_float2(top, sum);
+        }
+      }
+    }
+    fence_proxy_async_smem();  // the exchange's writes come before the next tile's bulk copies
+    __syncthreads();
+  }
+  if (tid == 0 && *abort_flag) atomicOr(&ffb_device_error_word, (uint32_t)ffb::ERR_ATTN_TIMEOUT);
+}
+
+// Joins the shares of one (row, head): one warp, four channels a lane.
+__global__ void __launch_bounds__(256) kv4_combine_kernel(const Args args) {
+  pdl_wait();
+  pdl_launch();
+  const int64_t n = (int64_t)args.seqs.T * args.HQ, at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (at >= n) return;
+  const int t = (int)(at / args.HQ), lane = threadIdx.x & 31;
+  if (t < __ldg(args.seqs.row_start) || t >= __ldg(args.seqs.row_start + args.seqs.B)) return;
+  float top = -INFINITY;
+  for (int s = lane; s < args.splits; s += 32) top = fmaxf(top, args.part_ml[(s * n + at) * 2]);
+  top = warp_max(top);
+  float sum = 0.f;
+  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int s = 0; s < args.splits; ++s) {
+    const float2 ml = *reinterpret_cast<const float2*>(args.part_ml + (s * n + at) * 2);
+    const float4 v = *reinterpret_cast<const float4*>(args.part_o + (s * n + at) * D + 4 * lane);
+    const float f = ml.x == -INFINITY && ml.y == 0.f ? 0.f : ex2(ml.x - top);
+    sum = fmaf(ml.y, f, sum);
+    y.x = fmaf(v.x, f, y.x);
+    y.y = fmaf(v.y, f, y.y);
+    y.z = fmaf(v.z, f, y.z);
+    y.w = fmaf(v.w, f, y.w);
+  }
+  const float r = sum == 0.f ? 0.f : 1.f / sum;
+  *reinterpret_cast<uint2*>(args.out + at * D + 4 * lane) = make_uint2(pack_bf16(y.x * r, y.y * r), pack_bf16(y.z * r, y.w * r));
+}
+
+// Shares of the page axis: enough CTAs for every SM, but a share keeps at least four pages (one
+// round of a CTA's page groups) and a join costs a launch.
+int plan_splits(int B, int HK, int tiles, int64_t pages) {
+  const int64_t base = (int64_t)B * HK * tiles;
+  const int sms = ffb::sm_count();
+  int best = 1;
+  double best_cost = 0;
+  for (int s = 1; s <= 64; ++s) {
+    if (s > 1 && pages < 4 * (int64_t)s) break;
+    const double waves = (double)((base * s + sms - 1) / sms);
+    const double rounds = (double)((pages + 4 * s - 1) / (4 * s));
+    const double cost = waves * (rounds * 0.5 + 2.0) + (s > 1 ? 2.0 + 0.02 * s : 0.0);  // microseconds, roughly
+    if (s == 1 || cost < best_cost) {
+      best = s;
+      best_cost = cost;
+    }
+  }
+  return best;
+}
+
+struct Plan {
+  int nt, tiles, splits;
+};
+Plan make_plan(int B, int HQ, int HK, int max_rows, int max_pages, int window, int sinks) {
+  Plan p;
+  const int64_t cols = (int64_t)max_rows * (HQ / HK);
+  p.nt = cols > 8 ? 2 : 1;
+  const int64_t tiles = (cols + 8 * p.nt - 1) / (8 * p.nt);
+  p.tiles = (int)(tiles < 4096 ? tiles : 4096);
+  int64_t pages = max_pages;
+  if (window > 0) {
+    const int64_t seen = ((int64_t)sinks + 63) / 64 + ((int64_t)window + max_rows + 126) / 64;
+    if (seen < pages) pages = seen;
+  }
+  p.splits = plan_splits(B, HK, p.tiles, pages);
+  return p;
+}
+
+}  // namespace
+
+extern "C" int64_t ffb_attention_kv4_workspace(int B, int T, int HQ, int HK, int max_rows, int max_pages, int window,
+                                               int sinks) {
+  if (B <= 0 || T <= 0 || HQ <= 0 || HK <= 0 || HQ % HK != 0 || max_rows <= 0 || max_pages <= 0 || window < 0 || sinks < 0)
+    return 0;
+  const Plan p = make_plan(B, HQ, HK, max_rows, max_pages, window, sinks);
+  return p.splits > 1 ? (int64_t)p.splits * T * HQ * (D + 2) * 4 : 0;
+}
+
+extern "C" int ffb_attention_kv4(const uint16_t* q, const uint8_t* pages, int num_pages, const int* page_table,
+                                 int64_t table_stride, int max_pages, const int* row_start, const int* ctx_len,
+                                 uint16_t* out, void* ws, int64_t ws_bytes, int B, int T, int max_rows, int HQ, int HK,
+                                 float scale, int window, int sinks, void* stream) {
+  const char* who = "ffb_attention_kv4";
+  int rc = ffb::kv4_check(who, pages, page_table, row_start, ctx_len, num_pages, table_stride, max_pages, B, T, HK);
+  if (rc) return rc;
+  FFB_REQUIRE(q && out, "%s: NULL pointer", who);
+  FFB_REQUIRE(HQ > 0 && HQ % HK == 0 && HQ <= 4096, "%s: bad heads HQ=%d HK=%d", who, HQ, HK);
+  FFB_REQUIRE(max_rows > 0 && max_rows <= T, "%s: max_rows %d (1..T=%d)", who, max_rows, T);
+  FFB_REQUIRE(isfinite(scale), "%s: scale must be finite", who);
+  FFB_REQUIRE(window >= 0 && sinks >= 0 && window <= (1 << 30) && sinks <= (1 << 30), "%s: window %d, sinks %d", who,
+              window, sinks);
+  FFB_REQUIRE((int64_t)T * HQ <= (1 << 30), "%s: T=%d x HQ=%d too large", who, T, HQ);
+  FFB_REQUIRE(sinks == 0 || window > 0, "%s: sinks without a window", who);
+  FFB_REQUIRE(ffb::aligned(q, 16) && ffb::aligned(out, 16), "%s: q and out must be 16-byte aligned", who);
+  const Plan p = make_plan(B, HQ, HK, max_rows, max_pages, window, sinks);
+  const int64_t need = p.splits > 1 ? (int64_t)p.splits * T * HQ * (D + 2) * 4 : 0;
+  FFB_REQUIRE(need == 0 || (ws && ws_bytes >= need && ffb::aligned(ws, 16)),
+              "%s: workspace of %lld bytes (16-byte aligned) needed, %lld given", who, (long long)need, (long long)ws_bytes);
+  const int64_t grid = (int64_t)B * HK * p.splits;
+  FFB_REQUIRE(grid <= 0x7fffffff, "%s: B=%d HK=%d too large", who, B, HK);
+  float* po = static_cast<float*>(ws);
+  Args a = {q, out, po, po ? po + (int64_t)p.splits * T * HQ * D : nullptr,
+            {const_cast<uint8_t*>(pages), page_table, row_start, ctx_len, num_pages, max_pages, B, T, HK, table_stride},
+            HQ, p.splits, window, sinks, scale * 1.4426950408889634f};
+  void (*kernel)(const Args) = p.nt == 1 ? kv4_attention_kernel<1> : kv4_attention_kernel<2>;
+  const int smem = p.nt == 1 ? smem_bytes<1>() : smem_bytes<2>();
+  cudaError_t e = ffb::set_smem_attr(reinterpret_cast<const void*>(kernel), smem);
+  if (e == cudaSuccess) e = ffb::launch(kernel, dim3((unsigned)grid, p.tiles), dim3(THREADS), smem, (cudaStream_t)stream, a);
+  if (e == cudaSuccess && p.splits > 1)
+    e = ffb::launch(kv4_combine_kernel, dim3((unsigned)(((int64_t)T * HQ + 7) / 8)), dim3(256), 0, (cudaStream_t)stream, a);
+  if (e != cudaSuccess) return ffb::fail(FFB_ECUDA, "%s: %s", who, cudaGetErrorString(e));
+  return FFB_OK;
+}

@@ -50,6 +50,7 @@ enum : uint32_t {
   ERR_ATTN_TIMEOUT = 1u << 2,
   ERR_GRID_SYNC_TIMEOUT = 1u << 3,
   ERR_PEER_TIMEOUT = 1u << 4,
+  ERR_KV4_PAGE = 1u << 5,  // a page id or position outside what a kv4 call was given
 };
 
 // Fills ffb_silu_table on this device once (stream-ordered, before the caller's next

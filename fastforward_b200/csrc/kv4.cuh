@@ -1,0 +1,68 @@
+// The 4-bit paged K/V cache: record layout, sequence bookkeeping and nibble arithmetic
+// shared by its writer, its reader and the attention kernels.
+//
+// A page holds 64 tokens.  Per (page, K/V head) one record of 9216 contiguous bytes, so one
+// bulk copy brings everything a tile of 64 keys needs:
+//   [0, 4096)     K codes, 64 bytes a token.  Byte 16 t + 4 j + e / 2, nibble e % 2 holds
+//                 channel 32 j + 8 t + e (t, j in 0..3, e in 0..7): 16 bytes hold, for each
+//                 scale group j, the eight channels that one lane of an MMA fragment needs.
+//   [4096, 8192)  V codes, 64 bytes a token: eight chunks of 8 bytes, chunk g at position
+//                 g ^ (token & 4); its nibble i holds channel 8 i + g.  The exchange of the
+//                 two halves for tokens 4..7 of eight spreads the fragment loads over all
+//                 shared-memory banks.
+//   [8192, 8704)  K scales bf16 [64][4];  [8704, 9216)  V scales bf16 [64][4].
+// A group of 32 channels has the scale s = the smallest number of five significant bits that
+// is >= max|x| / 7, codes q = rint(x / s) in -7..7, nibble q + 8.  Five bits times three fit
+// bf16's eight, so every held value q s is exact in bf16 and any kernel may multiply codes
+// and scales before or after its products with the same result.  The rounding up of s costs
+// at most 1/16 of a step and never clips.  max|x| < 2^-100 gives s = 0; a group with a
+// non-finite value (or one of 2^127 and more) gives s = NaN, so the row reads as NaN.
+#pragma once
+#include "common.cuh"
+
+namespace kv4 {
+
+constexpr int D = 128;
+constexpr int PAGE = FFB_KV4_PAGE;
+constexpr int RECORD = FFB_KV4_RECORD;
+constexpr int V_CODES = 4096, K_SCALES = 8192, V_SCALES = 8704;
+static_assert(PAGE == 64 && RECORD == 9216, "record layout");
+
+// What every entry is told about the cache and the rows of the call.
+struct Seqs {
+  uint8_t* pages;        // [num_pages][HK][RECORD]
+  const int* table;      // [B] rows of max_pages page ids, table_stride apart
+  const int* row_start;  // [B + 1]: rows [row_start[b], row_start[b + 1]) of the call are sequence b's newest
+  const int* ctx_len;    // [B]: tokens of sequence b with those rows
+  int num_pages, max_pages, B, T, HK;
+  int64_t table_stride;
+};
+
+// The sequence that row t belongs to, or -1 (rows before the first or behind the last).
+__device__ __forceinline__ int seq_of(const Seqs& s, int t) {
+  if (t < __ldg(s.row_start) || t >= __ldg(s.row_start + s.B)) return -1;
+  int lo = 0, hi = s.B;  // the first b with row_start[b + 1] > t
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (__ldg(s.row_start + mid + 1) > t) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo < s.B ? lo : -1;
+}
+
+// The record of (sequence b, position pos, head h), or NULL when the position is outside the
+// table or the page id outside the cache.
+__device__ __forceinline__ uint8_t* record_of(const Seqs& s, int b, int64_t pos, int h) {
+  if (pos < 0 || pos >= (int64_t)s.max_pages * PAGE) return nullptr;
+  const int page = __ldg(s.table + b * s.table_stride + pos / PAGE);
+  if (page < 0 || page >= s.num_pages) return nullptr;
+  return s.pages + ((int64_t)page * s.HK + h) * RECORD;
+}
+
+}  // namespace kv4
+
+namespace ffb {
+// The argument checks that every kv4 entry shares (host): FFB_OK or FFB_EINVAL with a message.
+int kv4_check(const char* who, const void* pages, const int* table, const int* row_start, const int* ctx_len,
+              int num_pages, int64_t table_stride, int max_pages, int B, int T, int HK);
+}  // namespace ffb

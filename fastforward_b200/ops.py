@@ -396,3 +396,102 @@ def vision_attention(q, k, v, d, scale):
     out = torch.empty(t, h * d, dtype=BF16, device=q.device)
     call("ffb_attention_full", ptr(q), ptr(k), ptr(v), ptr(out), t, h, int(d), float(scale), stream_ptr(q.device))
     return out
+
+
+# ---------------------------------------------------------------------------- 4-bit K/V cache
+
+def kv4_pages(num_pages, heads, device="cuda"):
+    """An empty 4-bit K/V cache: uint8 [num_pages, heads, 9216], one record of 64 tokens per
+    page and K/V head (see ffb_qk_norm_rope_kv4 in include/ffb200.h).  4.5 bits a value."""
+    _need(num_pages > 0 and heads > 0, "num_pages and heads must be positive")
+    return torch.zeros((num_pages, heads, L.KV4_RECORD), dtype=torch.uint8, device=device)
+
+
+def _kv4_place(pages, page_table, row_start, ctx_len):
+    """Checks the cache and the rows' description; returns the C entries' common arguments."""
+    _need(pages.is_cuda and page_table.is_cuda and row_start.is_cuda and ctx_len.is_cuda,
+          "CUDA tensors required (no CPU fallback)")
+    dev = pages.device
+    _need(page_table.device == dev and row_start.device == dev and ctx_len.device == dev, "tensors on one device")
+    _need(pages.dtype == torch.uint8 and pages.dim() == 3 and pages.shape[2] == L.KV4_RECORD and pages.is_contiguous(),
+          f"pages must be contiguous uint8 [pages, heads, {L.KV4_RECORD}]")
+    _need(page_table.dtype == row_start.dtype == ctx_len.dtype == torch.int32,
+          "page_table, row_start and ctx_len must be int32")
+    _need(page_table.dim() == 2 and (page_table.stride(1) == 1 or page_table.shape[1] == 1),
+          "page_table [B, width], unit last stride")
+    b = page_table.shape[0]
+    _need(row_start.shape == (b + 1,) and ctx_len.shape == (b,) and row_start.is_contiguous()
+          and ctx_len.is_contiguous(), f"row_start [{b + 1}] and ctx_len [{b}], contiguous")
+    return (ptr(pages), pages.shape[0], ptr(page_table), page_table.stride(0), page_table.shape[1]), (
+        ptr(row_start), ptr(ctx_len)), b
+
+
+def qk_pair_kv4(qkv, qn, kn, cos, sin, pages, page_table, row_start, ctx_len, out=None):
+    """`qk_pair` whose keys, and the values beside them, go into the 4-bit cache.  qkv [T,
+    (HQ + 2 HK) * 128] (any row stride that is a multiple of 4, unit last), cos / sin [T, 128]
+    (or [1, T, 128]).  Rows [row_start[b], row_start[b + 1]) are the newest tokens of sequence
+    b, whose cache holds ctx_len[b] tokens with them, in the pages of page_table[b].  Returns
+    the queries [HQ, T, 128] (`out`, or a new tensor; rows of no sequence are left as they
+    were).  Norm, rotation and quantisation run in one pass; the queries round once to bf16."""
+    place, rows, b = _kv4_place(pages, page_table, row_start, ctx_len)
+    _bf16_cuda(qkv, qn.weight, kn.weight, cos, sin)
+    _need(qkv.dim() == 2 and qkv.stride(1) == 1, "qkv [T, (HQ + 2 HK) * 128], unit last stride")
+    t, hk = qkv.shape[0], pages.shape[1]
+    hq = qkv.shape[1] // 128 - 2 * hk
+    _need(qkv.shape[1] % 128 == 0 and hq > 0 and hq % hk == 0, f"qkv width {qkv.shape[1]} for {hk} K/V heads")
+    _need(abs(qn.variance_epsilon - kn.variance_epsilon) < 1e-12, "q_norm and k_norm must share eps")
+    _need(qn.weight.shape == kn.weight.shape == (128,) and qn.weight.is_contiguous() and kn.weight.is_contiguous(),
+          "norm weights [128]")
+    _need(cos.numel() == sin.numel() == t * 128 and cos.shape[-1] == sin.shape[-1] == 128, "cos, sin [T, 128]")
+    _need(all(x.device == pages.device for x in (qkv, qn.weight, kn.weight, cos, sin)), "tensors on one device")
+    cos, sin = cos.contiguous(), sin.contiguous()
+    with torch.cuda.device(pages.device):
+        yq = torch.empty((hq, t, 128), device=qkv.device, dtype=BF16) if out is None else out
+        _need(yq.shape == (hq, t, 128) and yq.dtype == BF16 and yq.is_contiguous() and yq.device == pages.device,
+              f"out must be contiguous bf16 [{hq}, {t}, 128]")
+        if t:
+            call("ffb_qk_norm_rope_kv4", ptr(qkv), qkv.stride(0) if t > 1 else qkv.shape[1], ptr(qn.weight),
+                 ptr(kn.weight), float(qn.variance_epsilon), ptr(cos), ptr(sin), ptr(yq), *place, *rows, b, t, hq, hk,
+                 stream_ptr())
+    return yq
+
+
+def kv4_read(pages, page_table, row_start, ctx_len, rows):
+    """The newest rows as the 4-bit cache holds them: k, v [HK, rows, 128] bf16, exact.  To read
+    whole sequences, pass row_start with ctx_len's running sums."""
+    place, where, b = _kv4_place(pages, page_table, row_start, ctx_len)
+    hk = pages.shape[1]
+    with torch.cuda.device(pages.device):
+        k = torch.empty((hk, rows, 128), device=pages.device, dtype=BF16)
+        v = torch.empty_like(k)
+        if rows:
+            call("ffb_kv4_read", *place, *where, ptr(k), ptr(v), b, int(rows), hk, stream_ptr())
+    return k, v
+
+
+def attention_kv4(q, pages, page_table, row_start, ctx_len, scale, window=0, sinks=0, max_rows=None, out=None):
+    """Causal GQA attention of new rows over the 4-bit cache.  q [HQ, T, 128] as `qk_pair_kv4`
+    returns it (the rows' own keys are in the cache already); page_table, row_start, ctx_len as
+    there.  window > 0: a row at position p sees keys p - window + 1 .. p and the first `sinks`.
+    A row that sees nothing gets zeros.  max_rows: the most rows of one sequence in this call, if
+    known (it sizes the launch; default T, right for any mix).  Returns [T, HQ, 128] bf16 (`out`,
+    or a new tensor; rows of no sequence are left as they were)."""
+    place, where, b = _kv4_place(pages, page_table, row_start, ctx_len)
+    _bf16_cuda(q)
+    _need(q.dim() == 3 and q.shape[2] == 128 and q.is_contiguous(), "q must be contiguous [HQ, T, 128]")
+    hq, t, _ = q.shape
+    hk = pages.shape[1]
+    _need(hq > 0 and hq % hk == 0, f"{hq} query heads for {hk} K/V heads")
+    _need(q.device == pages.device, "tensors on one device")
+    most = t if max_rows is None else min(int(max_rows), t)
+    _need(most > 0 or t == 0, f"max_rows {max_rows}")
+    with torch.cuda.device(q.device):
+        y = torch.empty((t, hq, 128), device=q.device, dtype=BF16) if out is None else out
+        _need(y.shape == (t, hq, 128) and y.dtype == BF16 and y.is_contiguous() and y.device == q.device,
+              f"out must be contiguous bf16 [{t}, {hq}, 128]")
+        if t:
+            need = L.lib().ffb_attention_kv4_workspace(b, t, hq, hk, most, page_table.shape[1], int(window), int(sinks))
+            ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+            call("ffb_attention_kv4", ptr(q), *place, *where, ptr(y), ptr(ws), need, b, t, most, hq, hk, float(scale),
+                 int(window), int(sinks), stream_ptr())
+    return y

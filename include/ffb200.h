@@ -464,6 +464,60 @@ int ffb_vision_rope(const uint16_t* qkv, const float* cos, const float* sin, int
 int ffb_attention_full(const uint16_t* q, const uint16_t* k, const uint16_t* v, uint16_t* out,
                        int T, int H, int d, float scale, void* stream);
 
+/* ---------------------------------------------------------------- 4-bit K/V cache
+ * Keys and values kept between calls, at 4 bits a value, and the attention that reads them:
+ * follow-up questions over a cached image prefix, and token-by-token answers.  No counterpart
+ * in the reference (its K and V live within one forward pass).
+ *
+ * pages [num_pages][HK][FFB_KV4_RECORD] u8, 16-byte aligned: a page holds 64 tokens, and per
+ * K/V head one record of codes and scales (layout: csrc/kv4.cuh).  A group of 32 channels
+ * shares a scale s, the smallest number of five significant bits >= max|x| / 7 (bf16); a code
+ * is rint(x / s) in -7..7.  Every held value is exact in bf16.
+ *
+ * Every entry takes the same description of its T rows, on the device: row_start [B+1]
+ * (ascending): rows [row_start[b], row_start[b+1]) are sequence b's newest tokens (none, one
+ * or many); ctx_len [B]: sequence b's tokens with those rows, so row t has position
+ * ctx_len[b] - (row_start[b+1] - t); page_table: B rows of max_pages page ids, table_stride
+ * apart; entry i holds positions [64 i, 64 i + 64).  A page may be in several rows of the
+ * table (a shared prefix).  Rows before row_start[0] or from row_start[B] on belong to no
+ * sequence: they are not read and their outputs are left as they were.  A position outside
+ * the table or a page id outside [0, num_pages) is never dereferenced: it sets bit 5 of the
+ * device error word (ffb_device_error), a write of it is dropped, a read gives zeros, and
+ * attention leaves those keys out. */
+#define FFB_KV4_PAGE 64        /* tokens of a page                       */
+#define FFB_KV4_RECORD 9216    /* bytes of one page of one K/V head      */
+#define FFB_KV4_MAX_PAGES (1 << 24) /* widest page table (2^30 positions) */
+
+/* Per-head RMSNorm and rotation of queries and keys (as ffb_qk_norm_rope, but computed
+ * without intermediate bf16 roundings) with the keys and values quantised into the cache in
+ * the same pass.  qkv [T, (HQ+2HK)*128] bf16 rows, row_stride elements apart (a multiple of
+ * 4); q_norm, k_norm [128]; cos, sin [T, 128] bf16; yq [HQ, T, 128] bf16.  Two rows of a call
+ * must not share a position of a page (which of them is held is then not defined). */
+int ffb_qk_norm_rope_kv4(const uint16_t* qkv, int64_t row_stride, const uint16_t* q_norm,
+                         const uint16_t* k_norm, float eps, const uint16_t* cos, const uint16_t* sin,
+                         uint16_t* yq, uint8_t* pages, int num_pages, const int* page_table,
+                         int64_t table_stride, int max_pages, const int* row_start, const int* ctx_len,
+                         int B, int T, int HQ, int HK, void* stream);
+
+/* The rows of the call as the cache holds them: k, v [HK, T, 128] bf16 (exact). */
+int ffb_kv4_read(const uint8_t* pages, int num_pages, const int* page_table, int64_t table_stride,
+                 int max_pages, const int* row_start, const int* ctx_len, uint16_t* k, uint16_t* v, int B,
+                 int T, int HK, void* stream);
+
+/* Causal GQA attention of the rows over their sequences' cached keys (the rows' own among
+ * them: write them first).  q [HQ, T, 128], out [T, HQ*128] bf16, 16-byte aligned.  window > 0:
+ * row at position p sees keys j <= p with p - j < window or j < sinks; pages that no row sees
+ * are not read.  window 0: every key j <= p (sinks must be 0).  A row that sees no key gets
+ * zeros.  max_rows: the most rows that a sequence has in this call (1..T); it sizes the grid,
+ * longer sequences are still computed, only slower.  ws: ffb_attention_kv4_workspace(...)
+ * bytes, 16-byte aligned (NULL when 0), scratch of this call alone. */
+int ffb_attention_kv4(const uint16_t* q, const uint8_t* pages, int num_pages, const int* page_table,
+                      int64_t table_stride, int max_pages, const int* row_start, const int* ctx_len,
+                      uint16_t* out, void* ws, int64_t ws_bytes, int B, int T, int max_rows, int HQ, int HK,
+                      float scale, int window, int sinks, void* stream);
+int64_t ffb_attention_kv4_workspace(int B, int T, int HQ, int HK, int max_rows, int max_pages, int window,
+                                    int sinks);
+
 #ifdef __cplusplus
 }
 #endif
