@@ -47,21 +47,6 @@ constexpr int smem_bytes() {  // ring | Q fragments [NT][4][32] uint4 | offsets 
   return RING + NT * 4 * 512 + NT * 2 * 512 + BAR_BYTES + 128;
 }
 
-struct Args {
-  const uint16_t* q;  // [HQ, T, 128]
-  uint16_t* out;      // [T, HQ, 128]
-  float* part_o;      // [splits][T * HQ][128], relative to part_ml's maximum (splits > 1)
-  float* part_ml;     // [splits][T * HQ][2]
-  Seqs seqs;
-  int HQ, splits, window, sinks;
-  float scale_log2;
-};
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -74,45 +59,12 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-// Nibbles i and i + 4 of w as the bf16 pair (136 + code).
-__device__ __forceinline__ uint32_t pair136(uint32_t w, int i) { return ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u; }
-__device__ __forceinline__ uint32_t minus136(uint32_t w) {
-  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&w), __floats2bfloat162_rn(136.f, 136.f));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-__device__ __forceinline__ float lo_of(uint32_t w) { return __uint_as_float(w << 16); }
-__device__ __forceinline__ float hi_of(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                   smem_u32(dst)),
-               "l"(src), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
-}
 // The token of fragment row r (0..7): 2 <-> 3 and 6 <-> 7 trade places, so that the eight lanes
 // of a load phase meet rows of both parities and, with V's exchanged halves, all banks.
 __device__ __forceinline__ int token_of(int r) { return r ^ ((r >> 1) & 1); }
 
-// The pages that a tile of rows [first, last] (positions) reads: the first n_sink pages, then
-// [first_page, first_page + n - n_sink).
-struct PageSet {
-  int n, n_sink, first_page, first_key, kend;
-};
-__device__ __forceinline__ PageSet pages_of(int pos_lo, int pos_hi, int max_pages, int window, int sinks) {
-  PageSet s;
-  s.kend = min(pos_hi + 1, max_pages * PAGE);
-  s.first_key = window > 0 ? max(0, pos_lo - window + 1) : 0;
-  s.first_page = s.first_key / PAGE;
-  s.n_sink = window > 0 ? min((min(sinks, max(s.kend, 0)) + PAGE - 1) / PAGE, s.first_page) : 0;
-  s.n = s.kend > 0 ? s.n_sink + max(0, (s.kend + PAGE - 1) / PAGE - s.first_page) : 0;
-  return s;
-}
-
 template <int NT>
-__global__ void __launch_bounds__(THREADS, 1) kv4_attention_kernel(const Args args) {
+__global__ void __launch_bounds__(THREADS, 1) kv4_attention_kernel(const AttnArgs args) {
   constexpr int QT = 8 * NT;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
@@ -468,7 +420,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_kernel(const Args ar
 }
 
 // Joins the shares of one (row, head): one warp, four channels a lane.
-__global__ void __launch_bounds__(256) kv4_combine_kernel(const Args args) {
+// TC: the partials' columns are in the order that attention_kv4_tc.cu keeps them in.
+template <bool TC>
+__global__ void __launch_bounds__(256) kv4_combine_kernel(const AttnArgs args) {
   pdl_wait();
   pdl_launch();
   const int64_t n = (int64_t)args.seqs.T * args.HQ, at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -483,7 +437,15 @@ __global__ void __launch_bounds__(256) kv4_combine_kernel(const Args args) {
 #pragma unroll 4
   for (int s = 0; s < args.splits; ++s) {
     const float2 ml = *reinterpret_cast<const float2*>(args.part_ml + (s * n + at) * 2);
-    const float4 v = *reinterpret_cast<const float4*>(args.part_o + (s * n + at) * D + 4 * lane);
+    const float* row = args.part_o + (s * n + at) * D;
+    float4 v;
+    if constexpr (TC) {
+      // channel d = 64 half + 8 i + g sits in column 16 g + 8 half + 2 (i % 4) + i / 4
+      const int half = lane >> 4, i = (lane >> 1) & 7, col = 64 * (lane & 1) + 8 * half + 2 * (i & 3) + (i >> 2);
+      v = make_float4(row[col], row[col + 16], row[col + 32], row[col + 48]);
+    } else {
+      v = *reinterpret_cast<const float4*>(row + 4 * lane);
+    }
     const float f = ml.x == -INFINITY && ml.y == 0.f ? 0.f : ex2(ml.x - top);
     sum = fmaf(ml.y, f, sum);
     y.x = fmaf(v.x, f, y.x);
@@ -495,18 +457,25 @@ __global__ void __launch_bounds__(256) kv4_combine_kernel(const Args args) {
   *reinterpret_cast<uint2*>(args.out + at * D + 4 * lane) = make_uint2(pack_bf16(y.x * r, y.y * r), pack_bf16(y.z * r, y.w * r));
 }
 
-// Shares of the page axis: enough CTAs for every SM, but a share keeps at least four pages (one
-// round of a CTA's page groups) and a join costs a launch.
-int plan_splits(int B, int HK, int tiles, int64_t pages) {
-  const int64_t base = (int64_t)B * HK * tiles;
+// How a call is laid out.  kernel: 1 / 2 = the register path with 8 / 16 query columns a CTA,
+// TC = the tensor-memory path with 256.
+constexpr int TC = 3;
+struct Plan {
+  int kernel, tiles, splits;
+};
+
+// Shares of the page axis: enough CTAs for every SM, against the start and end of a CTA and the
+// join.  step: pages a CTA takes at a time; step_us, cta_us: what such a step and a CTA's start
+// and end take; join_us: a share's partials, written and read.
+int plan_splits(int64_t base, int64_t pages, int step, double step_us, double cta_us, double join_us) {
   const int sms = ffb::sm_count();
   int best = 1;
   double best_cost = 0;
   for (int s = 1; s <= 64; ++s) {
-    if (s > 1 && pages < 4 * (int64_t)s) break;
+    if (s > 1 && pages < (int64_t)step * s) break;
     const double waves = (double)((base * s + sms - 1) / sms);
-    const double rounds = (double)((pages + 4 * s - 1) / (4 * s));
-    const double cost = waves * (rounds * 0.5 + 2.0) + (s > 1 ? 2.0 + 0.02 * s : 0.0);  // microseconds, roughly
+    const double rounds = (double)((pages + step * s - 1) / (step * s));
+    const double cost = waves * (rounds * step_us + cta_us) + (s > 1 ? 2.0 + join_us * s : 0.0);
     if (s == 1 || cost < best_cost) {
       best = s;
       best_cost = cost;
@@ -515,31 +484,35 @@ int plan_splits(int B, int HK, int tiles, int64_t pages) {
   return best;
 }
 
-struct Plan {
-  int nt, tiles, splits;
-};
-Plan make_plan(int B, int HQ, int HK, int max_rows, int max_pages, int window, int sinks) {
+Plan make_plan(int B, int T, int HQ, int HK, int max_rows, int max_pages, int window, int sinks) {
   Plan p;
   const int64_t cols = (int64_t)max_rows * (HQ / HK);
-  p.nt = cols > 8 ? 2 : 1;
-  const int64_t tiles = (cols + 8 * p.nt - 1) / (8 * p.nt);
+  p.kernel = cols <= 8 ? 1 : cols <= 16 ? 2 : TC;
+  const int width = p.kernel == TC ? 256 : 8 * p.kernel;
+  const int64_t tiles = (cols + width - 1) / width;
   p.tiles = (int)(tiles < 4096 ? tiles : 4096);
   int64_t pages = max_pages;
   if (window > 0) {
     const int64_t seen = ((int64_t)sinks + 63) / 64 + ((int64_t)window + max_rows + 126) / 64;
     if (seen < pages) pages = seen;
   }
-  p.splits = plan_splits(B, HK, p.tiles, pages);
+  const double join = (double)T * HQ * (D + 2) * 4 * 2 / 5e6;  // written and read at about 5 TB/s
+  const int64_t base = (int64_t)B * HK * p.tiles;
+  p.splits = p.kernel == TC ? plan_splits(base, pages, 2, 1.4, 5.0, join) : plan_splits(base, pages, 4, 0.5, 2.0, join);
   return p;
 }
 
 }  // namespace
 
+namespace kv4 {
+cudaError_t launch_attention_tc(const AttnArgs& a, unsigned grid_x, unsigned tiles, cudaStream_t stream);
+}
+
 extern "C" int64_t ffb_attention_kv4_workspace(int B, int T, int HQ, int HK, int max_rows, int max_pages, int window,
                                                int sinks) {
   if (B <= 0 || T <= 0 || HQ <= 0 || HK <= 0 || HQ % HK != 0 || max_rows <= 0 || max_pages <= 0 || window < 0 || sinks < 0)
     return 0;
-  const Plan p = make_plan(B, HQ, HK, max_rows, max_pages, window, sinks);
+  const Plan p = make_plan(B, T, HQ, HK, max_rows, max_pages, window, sinks);
   return p.splits > 1 ? (int64_t)p.splits * T * HQ * (D + 2) * 4 : 0;
 }
 
@@ -559,22 +532,29 @@ extern "C" int ffb_attention_kv4(const uint16_t* q, const uint8_t* pages, int nu
   FFB_REQUIRE((int64_t)T * HQ <= (1 << 30), "%s: T=%d x HQ=%d too large", who, T, HQ);
   FFB_REQUIRE(sinks == 0 || window > 0, "%s: sinks without a window", who);
   FFB_REQUIRE(ffb::aligned(q, 16) && ffb::aligned(out, 16), "%s: q and out must be 16-byte aligned", who);
-  const Plan p = make_plan(B, HQ, HK, max_rows, max_pages, window, sinks);
+  const Plan p = make_plan(B, T, HQ, HK, max_rows, max_pages, window, sinks);
   const int64_t need = p.splits > 1 ? (int64_t)p.splits * T * HQ * (D + 2) * 4 : 0;
   FFB_REQUIRE(need == 0 || (ws && ws_bytes >= need && ffb::aligned(ws, 16)),
               "%s: workspace of %lld bytes (16-byte aligned) needed, %lld given", who, (long long)need, (long long)ws_bytes);
   const int64_t grid = (int64_t)B * HK * p.splits;
   FFB_REQUIRE(grid <= 0x7fffffff, "%s: B=%d HK=%d too large", who, B, HK);
   float* po = static_cast<float*>(ws);
-  Args a = {q, out, po, po ? po + (int64_t)p.splits * T * HQ * D : nullptr,
+  AttnArgs a = {q, out, po, po ? po + (int64_t)p.splits * T * HQ * D : nullptr,
             {const_cast<uint8_t*>(pages), page_table, row_start, ctx_len, num_pages, max_pages, B, T, HK, table_stride},
             HQ, p.splits, window, sinks, scale * 1.4426950408889634f};
-  void (*kernel)(const Args) = p.nt == 1 ? kv4_attention_kernel<1> : kv4_attention_kernel<2>;
-  const int smem = p.nt == 1 ? smem_bytes<1>() : smem_bytes<2>();
-  cudaError_t e = ffb::set_smem_attr(reinterpret_cast<const void*>(kernel), smem);
-  if (e == cudaSuccess) e = ffb::launch(kernel, dim3((unsigned)grid, p.tiles), dim3(THREADS), smem, (cudaStream_t)stream, a);
+  cudaStream_t st = (cudaStream_t)stream;
+  cudaError_t e;
+  if (p.kernel == TC) {
+    e = kv4::launch_attention_tc(a, (unsigned)grid, p.tiles, st);
+  } else {
+    void (*kernel)(const AttnArgs) = p.kernel == 1 ? kv4_attention_kernel<1> : kv4_attention_kernel<2>;
+    const int smem = p.kernel == 1 ? smem_bytes<1>() : smem_bytes<2>();
+    e = ffb::set_smem_attr(reinterpret_cast<const void*>(kernel), smem);
+    if (e == cudaSuccess) e = ffb::launch(kernel, dim3((unsigned)grid, p.tiles), dim3(THREADS), smem, st, a);
+  }
   if (e == cudaSuccess && p.splits > 1)
-    e = ffb::launch(kv4_combine_kernel, dim3((unsigned)(((int64_t)T * HQ + 7) / 8)), dim3(256), 0, (cudaStream_t)stream, a);
+    e = ffb::launch(p.kernel == TC ? kv4_combine_kernel<true> : kv4_combine_kernel<false>,
+                    dim3((unsigned)(((int64_t)T * HQ + 7) / 8)), dim3(256), 0, st, a);
   if (e != cudaSuccess) return ffb::fail(FFB_ECUDA, "%s: %s", who, cudaGetErrorString(e));
   return FFB_OK;
 }

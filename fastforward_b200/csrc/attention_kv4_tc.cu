@@ -1,0 +1,585 @@
+// Attention over the 4-bit paged K/V cache for many query rows a sequence (questions of tens
+// of rows over a cached prefix, chunks of hundreds), on tcgen05 with the codes dequantised in
+// shared memory.  Semantics and arguments: attention_kv4.cu, which plans and launches it.
+//
+// One CTA takes 256 query columns ((row, head of the group) pairs of one K/V head; two MMA
+// tiles of 128, A and B) and a share of the visible pages, two pages (128 keys) a block:
+//   warp 0       raw producer: one bulk copy of 9216 bytes a page into a ring of RAW pages
+//   warp 1       tensor memory, and the one thread that issues the MMAs:
+//                S = Q K^T (M 128, N 128, 8 steps of 16 channels), O += P V (8 steps of 16 keys,
+//                P read from tensor memory, V row-major)
+//   warps 4-11   softmax: four warps a tile, one thread a row
+//   warps 12-15  dequantisation: codes and scales of a block -> K and V tiles in bf16 (exact:
+//                five bits times three), 128-byte swizzled, in a ring of three 32 KB slots
+// The dequantisation is paid once per 256 columns, which is what makes the tensor cores worth
+// it over the register path of attention_kv4.cu.  Two query tiles let the MMAs of one run
+// while the other is in its softmax.  Tensor memory: S_A, S_B, O_A, O_B of 128 columns each;
+// P (bf16) overwrites the first 64 columns of its S.
+//
+// The running maximum of a row moves only when a score passes it by more than 8 (base 2), so
+// O stays in tensor memory and is rescaled there by the softmax warps on those rare blocks.
+// Channels are permuted inside the MMAs, never in memory: eight channels of a K word come out
+// of the nibble pairs as 0 4 1 5 2 6 3 7 and Q is laid out the same; the columns of O are
+// taken back to channels when they are stored.
+// A token whose V scale is not finite would poison rows that may not see it (0 x NaN), so its
+// V row is written as zeros and its K row as NaN: exactly the rows that see it become NaN.
+#include "kv4.cuh"
+#include "pdl.cuh"
+
+namespace {
+
+using namespace kv4;
+
+constexpr int THREADS = 512;
+constexpr int RAW = 6;                 // raw pages in flight
+constexpr int SLOTS = 3;               // 128-key K or V tiles
+constexpr int HALF = 128 * 128;        // 64 channels (K, Q) or columns (V) of 128 rows: 16 KB
+constexpr int TILE = 2 * HALF;
+constexpr int SMEM = 2 * TILE + SLOTS * TILE + RAW * RECORD + 512 + 1024;
+constexpr float LAZY = 8.f;
+
+// D[tmem] (+)= A[tmem] B[smem]^T, bf16.
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 r =
+      __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+// The eight codes of a word times the scale pair s, in the order 0 4 1 5 2 6 3 7.
+__device__ __forceinline__ uint4 dequant8(uint32_t w, uint32_t s) {
+  return make_uint4(mul2(minus136(pair136(w, 0)), s), mul2(minus136(pair136(w, 1)), s), mul2(minus136(pair136(w, 2)), s),
+                    mul2(minus136(pair136(w, 3)), s));
+}
+__device__ __forceinline__ bool not_finite2(uint32_t w) {  // either bf16 of the pair
+  return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+}
+// Named barrier over `count` threads that returns whether `pred` held in all of them.
+__device__ __forceinline__ bool all_of(int id, int count, bool pred) {
+  uint32_t out;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %3, 0;\n\t"
+      "barrier.cta.red.and.pred q, %1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(out)
+      : "r"(id), "r"(count), "r"((uint32_t)pred)
+      : "memory");
+  return out != 0;
+}
+// The channel of column (chunk, pos) of O: chunk = 2 g + half holds nibbles of V's chunk g.
+__device__ __forceinline__ int nibble_of(int pos) { return (pos >> 1) | ((pos & 1) << 2); }
+
+__global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const AttnArgs args) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sq = smem;                    // Q tiles A, B (at the end: the staged output rows)
+  uint8_t* slots = sq + 2 * TILE;
+  uint8_t* raw = slots + SLOTS * TILE;
+  uint64_t* raw_full = reinterpret_cast<uint64_t*>(raw + RAW * RECORD);
+  uint64_t* raw_empty = raw_full + RAW;
+  uint64_t* slot_full = raw_empty + RAW;
+  uint64_t* slot_empty = slot_full + SLOTS;
+  uint64_t* q_full = slot_empty + SLOTS;  // [2] per tile, as the rest
+  uint64_t* s_full = q_full + 2;
+  uint64_t* p_full = s_full + 2;
+  uint64_t* o_done = p_full + 2;
+  uint64_t* last = o_done + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(last + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile int* raw_bad = abort_flag + 1;  // [RAW]: the page is absent or its id outside the cache
+
+  const Seqs& sv = args.seqs;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int split = blockIdx.x % args.splits;
+  const int kvh = (blockIdx.x / args.splits) % sv.HK, b = blockIdx.x / (args.splits * sv.HK);
+  const int G = args.HQ / sv.HK;
+
+  if (tid == 0) {
+    for (int i = 0; i < RAW; ++i) {
+      mbar_init(&raw_full[i], 1);
+      mbar_init(&raw_empty[i], 4);
+    }
+    for (int i = 0; i < SLOTS; ++i) {
+      mbar_init(&slot_full[i], 4);
+      mbar_init(&slot_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 4);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_done[i], 1);
+    }
+    mbar_init(last, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  if (tid == 0) pdl_launch();
+
+  const int r0 = min(max(__ldg(sv.row_start + b), 0), sv.T);
+  const int r1 = min(max(__ldg(sv.row_start + b + 1), r0), sv.T);
+  const int S = r1 - r0, ctx = max(__ldg(sv.ctx_len + b), 0);
+  const int ncols = S * G;
+  const int* table = sv.table + b * sv.table_stride;
+  if (ctx > sv.max_pages * PAGE && S > 0 && tid == 0) atomicOr(&ffb_device_error_word, (uint32_t)ffb::ERR_KV4_PAGE);
+
+  // Every role walks the same query tiles and blocks; the counters run over all of them.
+  uint32_t blk0 = 0;           // blocks of the tiles before this one
+  uint32_t blkB0 = 0;          // those of them that tile B took part in
+  uint32_t tiles = 0, tilesB = 0;  // tiles with blocks
+  bool ok = true;
+
+  for (int c0 = (int)blockIdx.y * 256; c0 < ncols && ok; c0 += (int)gridDim.y * 256) {
+    const int clast = min(c0 + 256, ncols) - 1;
+    const bool two = clast >= c0 + 128;
+    const int pos_lo = ctx - S + c0 / G, pos_hi = ctx - S + clast / G;
+    const PageSet ps = pages_of(pos_lo, pos_hi, sv.max_pages, args.window, args.sinks);
+    const int pairs = (ps.n + 1) / 2;
+    const int i0 = 2 * (int)((int64_t)split * pairs / args.splits);
+    const int i1 = min(2 * (int)((int64_t)(split + 1) * pairs / args.splits), ps.n);
+    const int nblk = (i1 - i0 + 1) / 2;
+    auto page_index = [&](int i) { return i < ps.n_sink ? i : ps.first_page + i - ps.n_sink; };
+
+    if (warp == 0) {
+      // ---------------------------------------------------------------- raw pages
+      if (lane == 0) {
+        for (int i = 0; i < 2 * nblk; ++i) {
+          const uint32_t u = 2 * blk0 + i, s = u % RAW;
+          if (u >= RAW && !mbar_wait_bounded(&raw_empty[s], ((u / RAW) & 1u) ^ 1u, abort_flag)) {
+            *abort_flag = 1;
+            break;
+          }
+          int page = -1;
+          if (i0 + i < i1) {
+            page = __ldg(table + page_index(i0 + i));
+            if (page < 0 || page >= sv.num_pages) {
+              atomicOr(&ffb_device_error_word, (uint32_t)ffb::ERR_KV4_PAGE);
+              page = -1;
+            }
+          }
+          raw_bad[s] = page < 0;
+          if (page >= 0) {
+            mbar_arrive_expect_tx(&raw_full[s], RECORD);
+            bulk_load(raw + s * RECORD, sv.pages + ((int64_t)page * sv.HK + kvh) * RECORD, RECORD, &raw_full[s]);
+          } else {
+            mbar_arrive(&raw_full[s]);
+          }
+        }
+        // the copies have landed before this thread leaves (also when another role gave up)
+        volatile int never = 0;
+        if (*abort_flag) {
+          for (uint32_t i = 0; i < RAW; ++i) {
+            mbar_wait_bounded(&raw_full[i], 0, &never, 20000000ull);
+            mbar_wait_bounded(&raw_full[i], 1, &never, 20000000ull);
+          }
+        }
+      }
+    } else if (warp == 1) {
+      // ---------------------------------------------------------------- MMAs
+      if (lane == 0) {
+        constexpr uint32_t idesc_s = idesc_bf16(128, 128);
+        constexpr uint32_t idesc_o = idesc_bf16(128, 128) | (1u << 16);  // B (= V) MN-major
+        auto wait_slot = [&](uint32_t u) {
+          if (!mbar_wait_bounded(&slot_full[u % SLOTS], (u / SLOTS) & 1u, abort_flag)) return false;
+          tc_fence_after();
+          return true;
+        };
+        auto issue_s = [&](int x, uint32_t u) {
+          const uint32_t qa = smem_u32(sq + x * TILE), kb = smem_u32(slots + (u % SLOTS) * TILE);
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk)
+            umma_f16(tmem + 128 * x, umma_desc_sw128(qa + (kk >> 2) * HALF + (kk & 3) * 32),
+                     umma_desc_sw128(kb + (kk >> 2) * HALF + (kk & 3) * 32), idesc_s, kk > 0 ? 1u : 0u);
+          umma_commit(&s_full[x]);
+        };
+        auto issue_o = [&](int x, uint32_t u, bool first) {
+          const uint32_t vb = smem_u32(slots + (u % SLOTS) * TILE);
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk)
+            umma_f16_ts(tmem + 256 + 128 * x, tmem + 128 * x + 8 * kk, umma_desc_sw128_mn(vb + kk * 2048, HALF), idesc_o,
+                        (!first || kk > 0) ? 1u : 0u);
+          umma_commit(&o_done[x]);
+        };
+        bool go = true;
+        if (nblk > 0) {
+          go = mbar_wait_bounded(&q_full[0], tiles & 1u, abort_flag) &&
+               (!two || mbar_wait_bounded(&q_full[1], tilesB & 1u, abort_flag)) && wait_slot(2 * blk0);
+          if (go) {
+            issue_s(0, 2 * blk0);
+            if (two) issue_s(1, 2 * blk0);
+            umma_commit(&slot_empty[(2 * blk0) % SLOTS]);
+          }
+        }
+        for (int j = 0; j < nblk && go; ++j) {
+          const uint32_t uv = 2 * (blk0 + j) + 1, uk = uv + 1;
+          go = wait_slot(uv) && mbar_wait_bounded(&p_full[0], (blk0 + j) & 1u, abort_flag);
+          if (!go) break;
+          tc_fence_after();
+          issue_o(0, uv, j == 0);
+          const bool more = j + 1 < nblk;
+          if (more) {
+            go = wait_slot(uk);
+            if (!go) break;
+            issue_s(0, uk);
+          }
+          if (two) {
+            go = mbar_wait_bounded(&p_full[1], (blkB0 + j) & 1u, abort_flag);
+            if (!go) break;
+            tc_fence_after();
+            issue_o(1, uv, j == 0);
+          }
+          umma_commit(&slot_empty[uv % SLOTS]);
+          if (more) {
+            if (two) issue_s(1, uk);
+            umma_commit(&slot_empty[uk % SLOTS]);
+          }
+        }
+        if (!go) *abort_flag = 1;
+      }
+    } else if (warp >= 12) {
+      // ---------------------------------------------------------------- dequantisation
+      const int w = warp - 12;
+      for (int j = 0; j < nblk && ok; ++j) {
+#pragma unroll 1
+        for (int is_v = 0; is_v < 2; ++is_v) {
+          const uint32_t u = 2 * (blk0 + j) + is_v;
+          bool got = u < SLOTS || mbar_wait_bounded(&slot_empty[u % SLOTS], ((u / SLOTS) & 1u) ^ 1u, abort_flag);
+          got = __all_sync(0xffffffffu, got);  // one verdict for the warp
+          uint8_t* dst = slots + (u % SLOTS) * TILE;
+#pragma unroll 1
+          for (int a = 0; a < 2 && got; ++a) {
+            const uint32_t ur = 2 * (blk0 + j) + a, s = ur % RAW;
+            got = mbar_wait_bounded(&raw_full[s], (ur / RAW) & 1u, abort_flag);
+            got = __all_sync(0xffffffffu, got);
+            if (!got) break;
+            const uint8_t* rec = raw + s * RECORD;
+            const bool bad = raw_bad[s];
+            const int key0 = i0 + 2 * j + a < i1 ? page_index(i0 + 2 * j + a) * PAGE : 0;
+            // tokens past the newest row's position are held by nobody: whatever is there is not used
+            const int live = bad ? 0 : min(max(ps.kend - key0, 0), PAGE);
+#pragma unroll
+            for (int it = 0; it < 2; ++it) {
+              const int r8 = 8 * (w + 4 * it);  // this warp's eight tokens
+              if (!is_v) {
+                // token pairs (r, r ^ 5) x four chunks meet all banks on the load and on the store
+                const int k = lane >> 3, e = (lane >> 2) & 1, t = lane & 3;
+                const int r = r8 + (k ^ (e ? 5 : 0)) , row = 64 * a + r;
+                uint4 c = make_uint4(0u, 0u, 0u, 0u);
+                uint2 sc = make_uint2(0u, 0u);
+                if (r < live) {
+                  c = *reinterpret_cast<const uint4*>(rec + 64 * r + 16 * t);
+                  sc = *reinterpret_cast<const uint2*>(rec + K_SCALES + 8 * r);
+                  const uint2 vs = *reinterpret_cast<const uint2*>(rec + V_SCALES + 8 * r);
+                  if (not_finite2(vs.x) || not_finite2(vs.y)) sc = make_uint2(0x7fc07fc0u, 0x7fc07fc0u);
+                }
+                const uint32_t words[4] = {c.x, c.y, c.z, c.w};
+                const uint32_t scale[4] = {__byte_perm(sc.x, 0, 0x1010), __byte_perm(sc.x, 0, 0x3232),
+                                           __byte_perm(sc.y, 0, 0x1010), __byte_perm(sc.y, 0, 0x3232)};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                  const int chunk = 4 * (q & 1) + t;
+                  *reinterpret_cast<uint4*>(dst + (q >> 1) * HALF + row * 128 + ((chunk ^ (row & 7)) << 4)) =
+                      dequant8(words[q], scale[q]);
+                }
+              } else {
+                // tokens {0, 1, 6, 7} / {2, 3, 4, 5} of eight x two neighbouring 16-byte pairs
+                const int k = (lane >> 1) & 3, set = (lane >> 3) & 1, pair = 2 * (lane >> 4) + (lane & 1);
+                const int r = r8 + (set ? 2 + k : (k < 2 ? k : 4 + k)), row = 64 * a + r;
+                uint4 c = make_uint4(0u, 0u, 0u, 0u);
+                uint2 sc = make_uint2(0u, 0u);
+                if (r < live) {
+                  c = *reinterpret_cast<const uint4*>(rec + V_CODES + 64 * r + 16 * (pair ^ ((r & 4) >> 1)));
+                  sc = *reinterpret_cast<const uint2*>(rec + V_SCALES + 8 * r);
+                  if (not_finite2(sc.x) || not_finite2(sc.y)) sc = make_uint2(0u, 0u);
+                }
+                const uint32_t words[4] = {c.x, c.y, c.z, c.w};  // chunks 2 pair, 2 pair + 1, two words each
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                  const int chunk = 4 * (pair & 1) + q;
+                  *reinterpret_cast<uint4*>(dst + (pair >> 1) * HALF + row * 128 + ((chunk ^ (row & 7)) << 4)) =
+                      dequant8(words[q], (q & 1) ? sc.y : sc.x);
+                }
+              }
+            }
+          }
+          if (!got) {
+            ok = false;
+            *abort_flag = 1;
+            break;
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&slot_full[u % SLOTS]);
+            if (is_v) {
+              mbar_arrive(&raw_empty[(2 * (blk0 + j)) % RAW]);
+              mbar_arrive(&raw_empty[(2 * (blk0 + j) + 1) % RAW]);
+            }
+          }
+        }
+      }
+    } else if (warp >= 4) {
+      // ---------------------------------------------------------------- softmax
+      const int x = (warp - 4) >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+      if (x == 0 || two) {
+        const uint32_t base_blk = x ? blkB0 : blk0;
+        const int col = c0 + 128 * x + r;
+        const bool live_row = col <= clast;
+        const int row = live_row ? r0 + col / G : 0, head = live_row ? kvh * G + col % G : 0;
+        const int pos = live_row ? ctx - S + col / G : -1;
+        const float sc = fabsf(args.scale_log2);
+        // this warp's 32 rows of Q, negated for a negative scale (exact), eight channels a chunk in
+        // the order 0 4 1 5 2 6 3 7; sixteen lanes copy one row.  A tile without blocks has no queries:
+        // no product would keep its warps from staging output over rows that others still write
+        if (nblk > 0) {
+          const uint32_t flip = args.scale_log2 < 0.f ? 0x80008000u : 0u;
+          for (int k = 0; k < 32; k += 2) {
+            const int rr = quarter * 32 + k + (lane >> 4), cc = c0 + 128 * x + rr, ch = lane & 15;
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (cc <= clast)
+              v = __ldg(reinterpret_cast<const uint4*>(
+                  args.q + ((int64_t)(kvh * G + cc % G) * sv.T + r0 + cc / G) * D + 8 * ch));
+            // channels 8 ch .. of group ch / 4: chunk 4 (j & 1) + t of half j / 2 with j = ch / 4, t = ch % 4
+            const uint4 y = make_uint4(__byte_perm(v.x, v.z, 0x5410) ^ flip, __byte_perm(v.x, v.z, 0x7632) ^ flip,
+                                       __byte_perm(v.y, v.w, 0x5410) ^ flip, __byte_perm(v.y, v.w, 0x7632) ^ flip);
+            const int chunk = ch & 7;
+            *reinterpret_cast<uint4*>(sq + x * TILE + (ch >> 3) * HALF + rr * 128 + ((chunk ^ (rr & 7)) << 4)) = y;
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&q_full[x]);
+        }
+        const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
+        const uint32_t st = tmem + lane_addr + 128 * x, ot = tmem + lane_addr + 256 + 128 * x;
+        float m = -INFINITY, l = 0.f;
+        for (int j = 0; j < nblk; ++j) {
+          if (!__all_sync(0xffffffffu, mbar_wait_bounded(&s_full[x], (base_blk + j) & 1u, abort_flag) && !*abort_flag)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const int ia = i0 + 2 * j;
+          const bool has_b = ia + 1 < i1;
+          const int ka = page_index(ia) * PAGE, kb = has_b ? page_index(ia + 1) * PAGE : ps.kend;
+          auto seen_by_all = [&](int key0) {
+            return key0 + PAGE - 1 <= pos_lo && key0 + PAGE <= ps.kend &&
+                   (args.window == 0 || pos_hi - key0 < args.window || key0 + PAGE <= args.sinks);
+          };
+          const int pa = __ldg(table + page_index(ia)), pb = has_b ? __ldg(table + page_index(ia + 1)) : -1;
+          const bool good_a = pa >= 0 && pa < sv.num_pages, good_b = pb >= 0 && pb < sv.num_pages;
+          const bool whole = has_b && good_a && good_b && seen_by_all(ka) && seen_by_all(kb);
+          // columns of this row that count, per page: c <= hi and (c >= lo or c < sk)
+          const int top = min(pos, ps.kend - 1), low = args.window > 0 ? pos - args.window + 1 : 0;
+          const int hi[2] = {good_a ? top - ka : -1, good_b ? top - kb : -1};
+          const int lo[2] = {low - ka, low - kb}, sk[2] = {args.sinks - ka, args.sinks - kb};
+          float bmax = -INFINITY;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t v[32];
+            tmem_ld32_async(st + 32 * q, v);
+            tmem_wait_ld();
+            reg_fence(v);
+            if (whole) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) bmax = fmaxf(bmax, __uint_as_float(v[e]));
+            } else {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                const int c = 32 * (q & 1) + e;
+                if (c <= hi[q >> 1] && (c >= lo[q >> 1] || c < sk[q >> 1])) bmax = fmaxf(bmax, __uint_as_float(v[e]));
+              }
+            }
+          }
+          bmax *= sc;
+          if (!(bmax > -INFINITY)) bmax = -INFINITY;  // scale 0 of an empty row: 0 x -inf
+          const bool grow = bmax > m + LAZY;
+          if (__any_sync(0xffffffffu, grow)) {
+            const float nm = grow ? bmax : m;
+            const float alpha = grow ? ex2(m - nm) : 1.f;
+            l *= alpha;
+            m = nm;
+            if (j > 0) {
+              if (!__all_sync(0xffffffffu, mbar_wait_bounded(&o_done[x], (base_blk + j - 1) & 1u, abort_flag))) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+#pragma unroll 1
+              for (int q = 0; q < 8; ++q) {
+                uint32_t v[16];
+                tmem_ld16_async(ot + 16 * q, v);
+                tmem_wait_ld();
+                reg_fence(v);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * alpha);
+                tmem_st16(ot + 16 * q, v);
+              }
+              tmem_wait_st();
+            }
+          }
+          const float neg = m == -INFINITY ? 0.f : -m;
+          float sum[2] = {0.f, 0.f};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t v[32], p[16];
+            tmem_ld32_async(st + 32 * q, v);
+            tmem_wait_ld();
+            reg_fence(v);
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              float y0 = ex2(fmaf(__uint_as_float(v[e]), sc, neg)), y1 = ex2(fmaf(__uint_as_float(v[e + 1]), sc, neg));
+              if (!whole) {
+                const int c = 32 * (q & 1) + e, h = q >> 1;
+                if (!(c <= hi[h] && (c >= lo[h] || c < sk[h]))) y0 = 0.f;
+                if (!(c + 1 <= hi[h] && (c + 1 >= lo[h] || c + 1 < sk[h]))) y1 = 0.f;
+              }
+              sum[0] += y0;
+              sum[1] += y1;
+              p[e >> 1] = pack_bf16(y0, y1);
+            }
+            tmem_st16(st + 16 * q, p);
+          }
+          l += sum[0] + sum[1];
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[x]);
+        }
+        if (ok && nblk > 0)
+          ok = __all_sync(0xffffffffu, mbar_wait_bounded(&o_done[x], (base_blk + nblk - 1) & 1u, abort_flag) && !*abort_flag);
+        if (!ok) *abort_flag = 1;
+        if (ok) {
+          tc_fence_after();
+          const int64_t at = (int64_t)row * args.HQ + head;
+          if (args.splits > 1) {
+            // fp32 partials in the columns' order; kv4_combine takes them back to channels
+            const int64_t pt = (int64_t)split * sv.T * args.HQ + at;
+            if (live_row) *reinterpret_cast<float2*>(args.part_ml + pt * 2) = make_float2(m, l);
+#pragma unroll 1
+            for (int q = 0; q < 8; ++q) {
+              uint32_t v[16];
+              if (nblk > 0) {
+                tmem_ld16_async(ot + 16 * q, v);
+                tmem_wait_ld();
+                reg_fence(v);
+              } else {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) v[e] = 0u;
+              }
+              if (live_row)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  *reinterpret_cast<uint4*>(args.part_o + pt * D + 16 * q + 4 * e) =
+                      make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+            }
+          } else {
+            // rows staged over this warp's part of the Q tile (every S product has been read), words
+            // of two channels at word ^ (row % 32); 32 columns hold the channel pair 2 q of each 8
+            const float rl = l == 0.f ? 0.f : 1.f / l;
+            uint32_t* stage = reinterpret_cast<uint32_t*>(sq + x * TILE) + r * 64;
+#pragma unroll 1
+            for (int q = 0; q < 4; ++q) {
+              uint32_t v[32];
+              if (nblk > 0) {
+                tmem_ld32_async(ot + 32 * q, v);
+                tmem_wait_ld();
+                reg_fence(v);
+              } else {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) v[e] = 0u;
+              }
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {  // chunk 4 q (+ half) and 4 q + 2 (+ half): chunks g = 2 q and 2 q + 1 of V
+                const int half = e >> 3, d8 = 8 * half + nibble_of(e & 7);  // channels 8 d8 + 2 q, + 1
+                stage[(4 * d8 + q) ^ lane] = pack_bf16(__uint_as_float(v[e]) * rl, __uint_as_float(v[16 + e]) * rl);
+              }
+            }
+            __syncwarp();
+            for (int k = 0; k < 32; ++k) {
+              const int rr = quarter * 32 + k, cc = c0 + 128 * x + rr;
+              if (cc > clast) break;
+              const uint32_t* src = reinterpret_cast<const uint32_t*>(sq + x * TILE) + rr * 64;
+              uint32_t* dst = reinterpret_cast<uint32_t*>(args.out + ((int64_t)(r0 + cc / G) * args.HQ + kvh * G + cc % G) * D);
+              dst[lane] = src[lane ^ k];
+              dst[32 + lane] = src[32 + (lane ^ k)];
+            }
+            __syncwarp();
+          }
+          tc_fence_before();
+        }
+        // the four warps of a tile go on together (their staged rows and the next queries share the
+        // Q tile) and with one verdict, or leave together
+        ok = all_of(1 + x, 128, ok && !*abort_flag);
+      }
+    }
+    blk0 += nblk;
+    tiles += nblk > 0;
+    if (two) {
+      blkB0 += nblk;
+      tilesB += nblk > 0;
+    }
+  }
+
+  if (warp == 1 && lane == 0) {
+    // every MMA issued has completed before tensor and shared memory are released
+    volatile int never = 0;
+    umma_commit(last);
+    mbar_wait_bounded(last, 0, &never, 200000000ull);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (tid == 0 && *abort_flag) atomicOr(&ffb_device_error_word, (uint32_t)ffb::ERR_ATTN_TIMEOUT);
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace
+
+namespace kv4 {
+cudaError_t launch_attention_tc(const AttnArgs& a, unsigned grid_x, unsigned tiles, cudaStream_t stream) {
+  cudaError_t e = ffb::set_smem_attr(reinterpret_cast<const void*>(kv4_attention_tc_kernel), SMEM);
+  if (e == cudaSuccess)
+    e = ffb::launch(kv4_attention_tc_kernel, dim3(grid_x, tiles), dim3(THREADS), SMEM, stream, a);
+  return e;
+}
+}  // namespace kv4

@@ -59,6 +59,55 @@ __device__ __forceinline__ uint8_t* record_of(const Seqs& s, int b, int64_t pos,
   return s.pages + ((int64_t)page * s.HK + h) * RECORD;
 }
 
+// Arguments of the attention kernels.
+struct AttnArgs {
+  const uint16_t* q;  // [HQ, T, 128]
+  uint16_t* out;      // [T, HQ, 128]
+  float* part_o;      // [splits][T * HQ][128], relative to part_ml's maximum (splits > 1)
+  float* part_ml;     // [splits][T * HQ][2]
+  Seqs seqs;
+  int HQ, splits, window, sinks;
+  float scale_log2;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Nibbles i and i + 4 of w as the bf16 pair (136 + code).
+__device__ __forceinline__ uint32_t pair136(uint32_t w, int i) { return ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u; }
+__device__ __forceinline__ uint32_t minus136(uint32_t w) {
+  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&w), __floats2bfloat162_rn(136.f, 136.f));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float lo_of(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float hi_of(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+// The pages that a tile of rows [first, last] (positions) reads: the first n_sink pages, then
+// [first_page, first_page + n - n_sink).
+struct PageSet {
+  int n, n_sink, first_page, first_key, kend;
+};
+__device__ __forceinline__ PageSet pages_of(int pos_lo, int pos_hi, int max_pages, int window, int sinks) {
+  PageSet s;
+  s.kend = min(pos_hi + 1, max_pages * PAGE);
+  s.first_key = window > 0 ? max(0, pos_lo - window + 1) : 0;
+  s.first_page = s.first_key / PAGE;
+  s.n_sink = window > 0 ? min((min(sinks, max(s.kend, 0)) + PAGE - 1) / PAGE, s.first_page) : 0;
+  s.n = s.kend > 0 ? s.n_sink + max(0, (s.kend + PAGE - 1) / PAGE - s.first_page) : 0;
+  return s;
+}
+
 }  // namespace kv4
 
 namespace ffb {

@@ -170,6 +170,14 @@ def test_max_rows_is_only_a_hint(max_rows):
     _attend([40, 1, 7], [300, 64, 7], 8, 2, seed=9, max_rows=max_rows)
 
 
+@pytest.mark.parametrize("rows,ctx", [([300, 0, 7, 129], [500, 3, 7, 64]), ([65], [700]), ([64], [64]), ([513, 1], [515, 1300])])
+def test_long_chunks_with_a_small_hint(rows, ctx):
+    """More query tiles than the launch was sized for: a CTA takes several, one or both halves
+    of the last, tiles of no key among them."""
+    _attend(rows, ctx, 8, 2, seed=31, max_rows=5, lead=3, tail=2)
+    _attend(rows, ctx, 8, 2, seed=32, max_rows=5, window=70, sinks=5)
+
+
 def test_rows_that_see_nothing_are_zero():
     """More rows than the sequence holds: the first of them lie before its start."""
     got = _attend([4, 2], [1, 0], 4, 2, seed=2, max_rows=4)
