@@ -35,17 +35,23 @@ namespace {
 using namespace kv4;
 
 constexpr int GROUPS = 4;             // page streams of a CTA
-constexpr int THREADS = GROUPS * 128;
-constexpr int STAGES = 5;             // page records in flight per group
-constexpr int RING = GROUPS * STAGES * RECORD;
+constexpr int GW = 2;                 // warps of a group; each takes PAGE / GW tokens of a page
+constexpr int WARPS = GROUPS * GW;
+constexpr int THREADS = 32 * WARPS;
 constexpr int CS = D + 4;             // fp32 pitch of a column in the final exchange (spreads the banks)
-constexpr int BAR_BYTES = 2 * GROUPS * STAGES * 8 + GROUPS * STAGES * 4 + 16;
 constexpr float LAZY = 8.f;
 
 template <int NT>
-constexpr int smem_bytes() {  // ring | Q fragments [NT][4][32] uint4 | offsets [NT][2][32] float4 | barriers
-  return RING + NT * 4 * 512 + NT * 2 * 512 + BAR_BYTES + 128;
-}
+struct Shape {
+  // two CTAs an SM, so that one starts or ends while the other streams; 16 columns need the
+  // registers (64 sums a thread) and the stages of one
+  static constexpr int PER_SM = NT == 1 ? 2 : 1;
+  static constexpr int STAGES = NT == 1 ? 3 : 5;  // page records in flight per group
+  static constexpr int RING = GROUPS * STAGES * RECORD;
+  static constexpr int BARS = 2 * GROUPS * STAGES * 8 + GROUPS * STAGES * 4 + 16;
+  // ring | Q fragments [NT][4][32] uint4 | offsets [NT][2][32] float4 | barriers
+  static constexpr int SMEM = RING + NT * 4 * 512 + NT * 2 * 512 + BARS + 128;
+};
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
@@ -64,8 +70,8 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 __device__ __forceinline__ int token_of(int r) { return r ^ ((r >> 1) & 1); }
 
 template <int NT>
-__global__ void __launch_bounds__(THREADS, 1) kv4_attention_kernel(const AttnArgs args) {
-  constexpr int QT = 8 * NT;
+__global__ void __launch_bounds__(THREADS, Shape<NT>::PER_SM) kv4_attention_kernel(const AttnArgs args) {
+  constexpr int QT = 8 * NT, STAGES = Shape<NT>::STAGES, RING = Shape<NT>::RING;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
   uint4* sq = reinterpret_cast<uint4*>(smem + RING);                     // [NT][4][32]
@@ -77,15 +83,16 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_kernel(const AttnArg
 
   const Seqs& sq_ = args.seqs;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int group = warp >> 2, w4 = warp & 3, g = lane >> 2, t = lane & 3;
+  const int group = warp / GW, gw = warp % GW, g = lane >> 2, t = lane & 3;
   const int split = blockIdx.x % args.splits;
   const int kvh = (blockIdx.x / args.splits) % sq_.HK, b = blockIdx.x / (args.splits * sq_.HK);
   const int G = args.HQ / sq_.HK;
+  const bool producer = gw == 0 && lane == 0;
 
   if (tid == 0) {
     for (int i = 0; i < GROUPS * STAGES; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], 4);
+      mbar_init(&empty[i], GW);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -99,7 +106,12 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_kernel(const AttnArg
   const int S = r1 - r0, ctx = max(__ldg(sq_.ctx_len + b), 0);
   const int ncols = S * G;
   const int* table = sq_.table + b * sq_.table_stride;
-  uint32_t used = 0;  // stages this group has used so far (over all query tiles)
+  // The group's ring: the stage and phase parity of its next page to use; `fill` of the next to load.
+  int use = 0, fill = 0, freed = 0;
+  uint32_t use_ph = 0, freed_ph = 0;
+  uint64_t* gfull = full + group * STAGES;
+  uint64_t* gempty = empty + group * STAGES;
+  uint8_t* gring = smem + group * STAGES * RECORD;
   if (ctx > sq_.max_pages * PAGE && S > 0 && tid == 0) atomicOr(&ffb_device_error_word, (uint32_t)ffb::ERR_KV4_PAGE);
 
   for (int c0 = (int)blockIdx.y * QT; c0 < ncols; c0 += (int)gridDim.y * QT) {
@@ -108,31 +120,40 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_kernel(const AttnArg
     const PageSet ps = pages_of(pos_lo, pos_hi, sq_.max_pages, args.window, args.sinks);
     const int i0 = (int)((int64_t)split * ps.n / args.splits), i1 = (int)((int64_t)(split + 1) * ps.n / args.splits);
     const int cnt = max(0, (i1 - i0 - group + GROUPS - 1) / GROUPS);  // pages i0 + group + GROUPS k of this group
-    auto page_index = [&](int k) {
-      const int i = i0 + group + GROUPS * k;
-      return i < ps.n_sink ? i : ps.first_page + i - ps.n_sink;
-    };
-    auto issue = [&](int k) {  // one lane
-      const uint32_t u = used + k;
-      const int s = group * STAGES + u % STAGES;
-      const int page = __ldg(table + page_index(k));
+    // page indexes [whole_lo, whole_hi) are seen in full by every column
+    const int whole_key = args.window > 0 ? max(0, pos_hi - args.window + 1) : 0;
+    const int whole_lo = ps.n_sink + max(0, (whole_key + PAGE - 1) / PAGE - ps.first_page);
+    const int whole_hi = ps.n_sink + min(max(pos_lo + 1, 0), ps.kend) / PAGE - ps.first_page;
+    auto page_index = [&](int i) { return i < ps.n_sink ? i : ps.first_page + i - ps.n_sink; };
+    auto issue = [&](int k) {  // the producer lane
+      const int page = __ldg(table + page_index(i0 + group + GROUPS * k));
       const bool ok = page >= 0 && page < sq_.num_pages;
-      bad[s] = !ok;
+      bad[group * STAGES + fill] = !ok;
       if (ok) {
-        mbar_arrive_expect_tx(&full[s], RECORD);
-        bulk_load(smem + s * RECORD, sq_.pages + ((int64_t)page * sq_.HK + kvh) * RECORD, RECORD, &full[s]);
+        mbar_arrive_expect_tx(&gfull[fill], RECORD);
+        bulk_load(gring + fill * RECORD, sq_.pages + ((int64_t)page * sq_.HK + kvh) * RECORD, RECORD, &gfull[fill]);
       } else {
         atomicOr(&ffb_device_error_word, (uint32_t)ffb::ERR_KV4_PAGE);
-        mbar_arrive(&full[s]);
+        mbar_arrive(&gfull[fill]);
       }
+      fill = fill + 1 == STAGES ? 0 : fill + 1;
     };
-    int issued = 0;
-    if (w4 == 0 && lane == 0)
+    // the stage of the oldest page not known to be free: waits until its warps are done with it
+    auto reclaim = [&]() {
+      const bool done = mbar_wait_bounded(&gempty[freed], freed_ph, abort_flag);
+      if (++freed == STAGES) {
+        freed = 0;
+        freed_ph ^= 1u;
+      }
+      return done;
+    };
+    int issued = 0, reclaimed = 0;
+    if (producer)
       for (; issued < min(cnt, STAGES); ++issued) issue(issued);
 
     // query fragments of this tile, once per CTA: lane (g, t) of column tile n holds channels
     // 32 j + 8 t .. + 7 of column 8 n + g as the pairs (e, e + 4) that pair136 gives
-    for (int f = warp; f < 4 * NT; f += THREADS / 32) {
+    for (int f = warp; f < 4 * NT; f += WARPS) {
       const int n = f >> 2, j = f & 3;
       const int c = c0 + 8 * n + g;
       uint4 x = make_uint4(0u, 0u, 0u, 0u);
@@ -183,10 +204,10 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_kernel(const AttnArg
       pos[i] = c <= clast ? ctx - S + c / G : -1;
     }
 
-    // sixteen tokens of one page; MASKED: some column may not see some of them
-    auto tile = [&](const uint8_t* rec, int key0, auto masked_tag) {
+    // sixteen tokens of one page, from tok0 on; MASKED: some column may not see some of them
+    auto tile = [&](const uint8_t* rec, int tok0, int key0, auto masked_tag) {
       constexpr bool MASKED = decltype(masked_tag)::value;
-      const int ra = 16 * w4 + token_of(g), rb = ra + 8;  // tokens of fragment rows g and g + 8
+      const int ra = tok0 + token_of(g), rb = ra + 8;  // tokens of fragment rows g and g + 8
       float s[NT][4];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
@@ -207,24 +228,22 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_kernel(const AttnArg
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             uint32_t q0, q1, q2, q3;
-            float c[4];
+            float c[4] = {0.f, 0.f, 0.f, 0.f}, d0, d1;
             if constexpr (NT == 1) {
               q0 = qf[4 * j]; q1 = qf[4 * j + 1]; q2 = qf[4 * j + 2]; q3 = qf[4 * j + 3];
-              c[0] = off[2 * j]; c[1] = off[2 * j + 1];
+              d0 = off[2 * j]; d1 = off[2 * j + 1];
             } else {
               const uint4 x = sq[(n * 4 + j) * 32 + lane];
               q0 = x.x; q1 = x.y; q2 = x.z; q3 = x.w;
               const float2 y = reinterpret_cast<const float2*>(soff)[((n * 2 + (j >> 1)) * 32 + lane) * 2 + (j & 1)];
-              c[0] = y.x; c[1] = y.y;
+              d0 = y.x; d1 = y.y;
             }
-            c[2] = c[0];
-            c[3] = c[1];
             mma16816(c, a0, a1, a2, a3, q0, q1);
             mma16816(c, a4, a5, a6, a7, q2, q3);
-            s[n][0] = fmaf(c[0], fa[j], s[n][0]);
-            s[n][1] = fmaf(c[1], fa[j], s[n][1]);
-            s[n][2] = fmaf(c[2], fb[j], s[n][2]);
-            s[n][3] = fmaf(c[3], fb[j], s[n][3]);
+            s[n][0] = fmaf(c[0] + d0, fa[j], s[n][0]);
+            s[n][1] = fmaf(c[1] + d1, fa[j], s[n][1]);
+            s[n][2] = fmaf(c[2] + d0, fb[j], s[n][2]);
+            s[n][3] = fmaf(c[3] + d1, fb[j], s[n][3]);
           }
         }
       }
@@ -288,7 +307,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_kernel(const AttnArg
         }
       }
       // V^T fragments: columns 2t, 2t+1, 2t+8, 2t+9 of the MMA are these four tokens
-      const int ta = 16 * w4 + token_of(2 * t), tb = 16 * w4 + token_of(2 * t + 1);
+      const int ta = tok0 + token_of(2 * t), tb = tok0 + token_of(2 * t + 1);
       const uint8_t* v = rec + V_CODES + 8 * (g ^ (4 * (t >> 1)));
       const uint2 v0 = *reinterpret_cast<const uint2*>(v + 64 * ta), v1 = *reinterpret_cast<const uint2*>(v + 64 * tb);
       const uint2 v2 = *reinterpret_cast<const uint2*>(v + 64 * ta + 512), v3 = *reinterpret_cast<const uint2*>(v + 64 * tb + 512);
@@ -313,44 +332,52 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_kernel(const AttnArg
 
     bool ok = true;
     for (int k = 0; k < cnt; ++k) {
-      const uint32_t u = used + k;
-      const int s = group * STAGES + u % STAGES;
       // one verdict for the warp: its lanes stay together whatever each of them saw
-      if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full[s], (u / STAGES) & 1u, abort_flag))) {
+      if (!__all_sync(0xffffffffu, mbar_try_wait(&gfull[use], use_ph)) &&
+          !__all_sync(0xffffffffu, mbar_wait_bounded(&gfull[use], use_ph, abort_flag))) {
         ok = false;
         break;
       }
-      const int key0 = page_index(k) * PAGE;
-      if (!bad[s] && key0 + 16 * w4 < ps.kend) {
-        const uint8_t* rec = smem + s * RECORD;
-        const bool whole = key0 + PAGE - 1 <= pos_lo && key0 + PAGE <= ps.kend &&
-                           (args.window == 0 || pos_hi - key0 < args.window || key0 + PAGE <= args.sinks);
-        if (whole) tile(rec, key0, std::integral_constant<bool, false>{});
-        else tile(rec, key0, std::integral_constant<bool, true>{});
+      const int i = i0 + group + GROUPS * k;
+      if (!bad[group * STAGES + use]) {
+        const uint8_t* rec = gring + use * RECORD;
+        constexpr int TOK = PAGE / GW;
+        if (i >= whole_lo && i < whole_hi) {
+#pragma unroll 1
+          for (int a = 0; a < TOK; a += 16) tile(rec, TOK * gw + a, 0, std::integral_constant<bool, false>{});
+        } else {
+          const int key0 = page_index(i) * PAGE;
+#pragma unroll 1
+          for (int a = 0; a < TOK; a += 16)
+            if (key0 + TOK * gw + a < ps.kend) tile(rec, TOK * gw + a, key0, std::integral_constant<bool, true>{});
+        }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[s]);
-      // refill the stage of the page before this one (its four warps are about to be done)
-      if (w4 == 0 && lane == 0 && k > 0 && issued < cnt) {
-        const uint32_t f = used + k - 1;
-        if (mbar_wait_bounded(&empty[group * STAGES + f % STAGES], (f / STAGES) & 1u, abort_flag)) issue(issued++);
+      if (lane == 0) mbar_arrive(&gempty[use]);
+      if (++use == STAGES) {
+        use = 0;
+        use_ph ^= 1u;
+      }
+      // refill the stage of the page before this one (the group's warps are about to be done with it)
+      if (producer && k > 0 && issued < cnt) {
+        if (reclaim()) issue(issued++);
         else *abort_flag = 1;  // the waits for the pages never issued give up on it
+        ++reclaimed;
       }
     }
-    // every stage of this tile is waited for before the ring is used again: `used` counts
-    // whole tiles, and the stages not waited on as empty above are drained here
     if (!ok) *abort_flag = 1;
-    if (w4 == 0 && lane == 0) {
+    if (producer) {
       volatile int never = 0;
       if (*abort_flag) {  // copies in flight must land before the CTA leaves
-        for (int k = max(0, issued - STAGES); k < issued; ++k)
-          mbar_wait_bounded(&full[group * STAGES + (used + k) % STAGES], ((used + k) / STAGES) & 1u, &never, 200000000ull);
-      } else {
-        for (int k = max(0, cnt - STAGES); k < cnt; ++k)
-          if (!mbar_wait_bounded(&empty[group * STAGES + (used + k) % STAGES], ((used + k) / STAGES) & 1u, abort_flag)) *abort_flag = 1;
+        for (int i = 0; i < STAGES; ++i) {
+          mbar_wait_bounded(&gfull[i], 0, &never, 20000000ull);
+          mbar_wait_bounded(&gfull[i], 1, &never, 20000000ull);
+        }
+      } else {  // every stage free again: the ring is used for the exchange, then for the next tile
+        for (; reclaimed < cnt; ++reclaimed)
+          if (!reclaim()) *abort_flag = 1;
       }
     }
-    used += cnt;
 #pragma unroll
     for (int i = 0; i < 2 * NT; ++i) {
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 4);
@@ -359,10 +386,10 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_kernel(const AttnArg
     }
     __syncthreads();  // all pages consumed: the ring becomes the exchange buffer
     if (*abort_flag) break;  // uniform: read after the barrier that follows every write
-    // [16 warps][QT] maxima, sums, then [16 warps][QT][CS] outputs; NT = 2 in two rounds of 8 columns
+    // [WARPS][QT] maxima, sums, then [WARPS][8][CS] outputs, eight columns at a time
     float* xm = reinterpret_cast<float*>(smem);
-    float* xl = xm + 16 * QT;
-    float* xo = xl + 16 * QT;
+    float* xl = xm + WARPS * QT;
+    float* xo = xl + WARPS * QT;
     if (g == 0) {
 #pragma unroll
       for (int i = 0; i < 2 * NT; ++i) {
@@ -383,33 +410,36 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_kernel(const AttnArg
         dst[CS + 8] = o[mt][n][3];
       }
       __syncthreads();
-      // 8 columns x 128 channels over 512 threads: two neighbouring channels a thread
-      const int c = tid >> 6, d = 2 * (tid & 63);
+      // 8 columns x 128 channels over 256 threads: four neighbouring channels a thread, a warp a column
+      const int c = warp, d = 4 * lane;
       const int col = c0 + 8 * n + c;
       if (col <= clast) {
         float top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < 16; ++w) top = fmaxf(top, xm[w * QT + 8 * n + c]);
-        float sum = 0.f, y0 = 0.f, y1 = 0.f;
+        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, xm[w * QT + 8 * n + c]);
+        float sum = 0.f;
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < 16; ++w) {
-          const float mw = xm[w * QT + 8 * n + c];
-          if (mw == -INFINITY && xl[w * QT + 8 * n + c] == 0.f) continue;  // this warp saw nothing of the row
+        for (int w = 0; w < WARPS; ++w) {
+          const float mw = xm[w * QT + 8 * n + c], lw = xl[w * QT + 8 * n + c];
+          if (mw == -INFINITY && lw == 0.f) continue;  // this warp saw nothing of the row
           const float f = ex2(mw - top);
-          const float2 v = *reinterpret_cast<const float2*>(xo + (w * 8 + c) * CS + d);
-          sum = fmaf(xl[w * QT + 8 * n + c], f, sum);
-          y0 = fmaf(v.x, f, y0);
-          y1 = fmaf(v.y, f, y1);
+          const float4 v = *reinterpret_cast<const float4*>(xo + (w * 8 + c) * CS + d);
+          sum = fmaf(lw, f, sum);
+          y.x = fmaf(v.x, f, y.x);
+          y.y = fmaf(v.y, f, y.y);
+          y.z = fmaf(v.z, f, y.z);
+          y.w = fmaf(v.w, f, y.w);
         }
         const int row = r0 + col / G, h = kvh * G + col % G;
         const int64_t at = (int64_t)row * args.HQ + h;
         if (args.splits == 1) {
           const float r = sum == 0.f ? 0.f : 1.f / sum;  // nothing visible: zeros
-          *reinterpret_cast<uint32_t*>(args.out + at * D + d) = pack_bf16(y0 * r, y1 * r);
+          *reinterpret_cast<uint2*>(args.out + at * D + d) = make_uint2(pack_bf16(y.x * r, y.y * r), pack_bf16(y.z * r, y.w * r));
         } else {
           const int64_t pt = (int64_t)split * sq_.T * args.HQ + at;
-          *reinterpret_cast<float2*>(args.part_o + pt * D + d) = make_float2(y0, y1);
-          if (d == 0) *reinterpret_cast<float2*>(args.part_ml + pt * 2) = make_float2(top, sum);
+          *reinterpret_cast<float4*>(args.part_o + pt * D + d) = y;
+          if (lane == 0) *reinterpret_cast<float2*>(args.part_ml + pt * 2) = make_float2(top, sum);
         }
       }
     }
@@ -465,18 +495,21 @@ struct Plan {
 };
 
 // Shares of the page axis: enough CTAs for every SM, against the start and end of a CTA and the
-// join.  step: pages a CTA takes at a time; step_us, cta_us: what such a step and a CTA's start
-// and end take; join_us: a share's partials, written and read.
-int plan_splits(int64_t base, int64_t pages, int step, double step_us, double cta_us, double join_us) {
-  const int sms = ffb::sm_count();
+// join.  slots: CTAs that run at once; step: pages a CTA takes at a time; step_us, cta_us: what
+// such a step and a CTA's start and end take; join_us: a share's partials, written and read.
+// Only share counts that fill whole waves are compared.
+int plan_splits(int64_t base, int64_t pages, int slots, int step, double step_us, double cta_us, double join_us) {
   int best = 1;
   double best_cost = 0;
-  for (int s = 1; s <= 64; ++s) {
-    if (s > 1 && pages < (int64_t)step * s) break;
-    const double waves = (double)((base * s + sms - 1) / sms);
+  for (int wave = 0; wave <= 4; ++wave) {
+    int64_t fit = wave == 0 ? 1 : wave * slots / base;
+    if (fit > pages / step) fit = pages / step;
+    const int s = wave == 0 ? 1 : (int)(fit < 64 ? fit : 64);
+    if (s < 1) continue;
+    const double waves = (double)((base * s + slots - 1) / slots);
     const double rounds = (double)((pages + step * s - 1) / (step * s));
     const double cost = waves * (rounds * step_us + cta_us) + (s > 1 ? 2.0 + join_us * s : 0.0);
-    if (s == 1 || cost < best_cost) {
+    if (wave == 0 || cost < best_cost) {
       best = s;
       best_cost = cost;
     }
@@ -498,7 +531,9 @@ Plan make_plan(int B, int T, int HQ, int HK, int max_rows, int max_pages, int wi
   }
   const double join = (double)T * HQ * (D + 2) * 4 * 2 / 5e6;  // written and read at about 5 TB/s
   const int64_t base = (int64_t)B * HK * p.tiles;
-  p.splits = p.kernel == TC ? plan_splits(base, pages, 2, 1.4, 5.0, join) : plan_splits(base, pages, 4, 0.5, 2.0, join);
+  const int sms = ffb::sm_count();
+  p.splits = p.kernel == TC ? plan_splits(base, pages, sms, 2, 1.4, 5.0, join)
+                            : plan_splits(base, pages, (p.kernel == 1 ? Shape<1>::PER_SM : Shape<2>::PER_SM) * sms, GROUPS, 0.9, 3.0, join);
   return p;
 }
 
@@ -548,7 +583,7 @@ extern "C" int ffb_attention_kv4(const uint16_t* q, const uint8_t* pages, int nu
     e = kv4::launch_attention_tc(a, (unsigned)grid, p.tiles, st);
   } else {
     void (*kernel)(const AttnArgs) = p.kernel == 1 ? kv4_attention_kernel<1> : kv4_attention_kernel<2>;
-    const int smem = p.kernel == 1 ? smem_bytes<1>() : smem_bytes<2>();
+    const int smem = p.kernel == 1 ? Shape<1>::SMEM : Shape<2>::SMEM;
     e = ffb::set_smem_attr(reinterpret_cast<const void*>(kernel), smem);
     if (e == cudaSuccess) e = ffb::launch(kernel, dim3((unsigned)grid, p.tiles), dim3(THREADS), smem, st, a);
   }

@@ -409,21 +409,37 @@ def kv4_pages(num_pages, heads, device="cuda"):
 
 def _kv4_place(pages, page_table, row_start, ctx_len):
     """Checks the cache and the rows' description; returns the C entries' common arguments."""
-    _need(pages.is_cuda and page_table.is_cuda and row_start.is_cuda and ctx_len.is_cuda,
-          "CUDA tensors required (no CPU fallback)")
     dev = pages.device
-    _need(page_table.device == dev and row_start.device == dev and ctx_len.device == dev, "tensors on one device")
-    _need(pages.dtype == torch.uint8 and pages.dim() == 3 and pages.shape[2] == L.KV4_RECORD and pages.is_contiguous(),
-          f"pages must be contiguous uint8 [pages, heads, {L.KV4_RECORD}]")
-    _need(page_table.dtype == row_start.dtype == ctx_len.dtype == torch.int32,
-          "page_table, row_start and ctx_len must be int32")
-    _need(page_table.dim() == 2 and (page_table.stride(1) == 1 or page_table.shape[1] == 1),
-          "page_table [B, width], unit last stride")
-    b = page_table.shape[0]
-    _need(row_start.shape == (b + 1,) and ctx_len.shape == (b,) and row_start.is_contiguous()
-          and ctx_len.is_contiguous(), f"row_start [{b + 1}] and ctx_len [{b}], contiguous")
-    return (ptr(pages), pages.shape[0], ptr(page_table), page_table.stride(0), page_table.shape[1]), (
-        ptr(row_start), ptr(ctx_len)), b
+    if not (pages.is_cuda and page_table.device == row_start.device == ctx_len.device == dev):
+        _need(False, "CUDA tensors of one device required (no CPU fallback)")
+    if not (pages.dtype is torch.uint8 and pages.dim() == 3 and pages.shape[2] == L.KV4_RECORD and pages.is_contiguous()):
+        _need(False, f"pages must be contiguous uint8 [pages, heads, {L.KV4_RECORD}]")
+    if not (page_table.dtype is row_start.dtype is ctx_len.dtype is torch.int32):
+        _need(False, "page_table, row_start and ctx_len must be int32")
+    if page_table.dim() != 2 or (page_table.stride(1) != 1 and page_table.shape[1] != 1):
+        _need(False, "page_table [B, width], unit last stride")
+    b, width = page_table.shape
+    if not (row_start.shape == (b + 1,) and ctx_len.shape == (b,) and row_start.is_contiguous() and ctx_len.is_contiguous()):
+        _need(False, f"row_start [{b + 1}] and ctx_len [{b}], contiguous")
+    return (pages.data_ptr(), pages.shape[0], page_table.data_ptr(), page_table.stride(0), width), (
+        row_start.data_ptr(), ctx_len.data_ptr()), b
+
+
+def _kv4_call(device, name, *args):
+    """`call` on `device`'s current stream, with that device current."""
+    if torch._C._cuda_getDevice() == device.index:
+        call(name, *args, L.raw_stream(device))
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, L.raw_stream(device))
+
+
+def _kv4_out(out, shape, device):
+    if out is None:
+        return torch.empty(shape, device=device, dtype=BF16)
+    _need(out.shape == shape and out.dtype == BF16 and out.is_contiguous() and out.device == device,
+          f"out must be contiguous bf16 {list(shape)}")
+    return out
 
 
 def qk_pair_kv4(qkv, qn, kn, cos, sin, pages, page_table, row_start, ctx_len, out=None):
@@ -434,25 +450,22 @@ def qk_pair_kv4(qkv, qn, kn, cos, sin, pages, page_table, row_start, ctx_len, ou
     the queries [HQ, T, 128] (`out`, or a new tensor; rows of no sequence are left as they
     were).  Norm, rotation and quantisation run in one pass; the queries round once to bf16."""
     place, rows, b = _kv4_place(pages, page_table, row_start, ctx_len)
-    _bf16_cuda(qkv, qn.weight, kn.weight, cos, sin)
+    qw, kw = qn.weight, kn.weight
+    _bf16_cuda(qkv, qw, kw, cos, sin)
     _need(qkv.dim() == 2 and qkv.stride(1) == 1, "qkv [T, (HQ + 2 HK) * 128], unit last stride")
-    t, hk = qkv.shape[0], pages.shape[1]
-    hq = qkv.shape[1] // 128 - 2 * hk
-    _need(qkv.shape[1] % 128 == 0 and hq > 0 and hq % hk == 0, f"qkv width {qkv.shape[1]} for {hk} K/V heads")
+    (t, width), hk, dev = qkv.shape, pages.shape[1], pages.device
+    hq = width // 128 - 2 * hk
+    _need(width % 128 == 0 and hq > 0 and hq % hk == 0, "qkv width does not fit the cache's K/V heads")
     _need(abs(qn.variance_epsilon - kn.variance_epsilon) < 1e-12, "q_norm and k_norm must share eps")
-    _need(qn.weight.shape == kn.weight.shape == (128,) and qn.weight.is_contiguous() and kn.weight.is_contiguous(),
-          "norm weights [128]")
+    _need(qw.shape == kw.shape == (128,) and qw.is_contiguous() and kw.is_contiguous(), "norm weights [128]")
     _need(cos.numel() == sin.numel() == t * 128 and cos.shape[-1] == sin.shape[-1] == 128, "cos, sin [T, 128]")
-    _need(all(x.device == pages.device for x in (qkv, qn.weight, kn.weight, cos, sin)), "tensors on one device")
-    cos, sin = cos.contiguous(), sin.contiguous()
-    with torch.cuda.device(pages.device):
-        yq = torch.empty((hq, t, 128), device=qkv.device, dtype=BF16) if out is None else out
-        _need(yq.shape == (hq, t, 128) and yq.dtype == BF16 and yq.is_contiguous() and yq.device == pages.device,
-              f"out must be contiguous bf16 [{hq}, {t}, 128]")
-        if t:
-            call("ffb_qk_norm_rope_kv4", ptr(qkv), qkv.stride(0) if t > 1 else qkv.shape[1], ptr(qn.weight),
-                 ptr(kn.weight), float(qn.variance_epsilon), ptr(cos), ptr(sin), ptr(yq), *place, *rows, b, t, hq, hk,
-                 stream_ptr())
+    _need(qkv.device == qw.device == kw.device == cos.device == sin.device == dev, "tensors on one device")
+    cos, sin = cos.contiguous(), sin.contiguous()  # held until the launch is enqueued
+    yq = _kv4_out(out, (hq, t, 128), dev)
+    if t:
+        _kv4_call(dev, "ffb_qk_norm_rope_kv4", qkv.data_ptr(), qkv.stride(0) if t > 1 else width, qw.data_ptr(),
+                  kw.data_ptr(), qn.variance_epsilon, cos.data_ptr(), sin.data_ptr(), yq.data_ptr(), *place, *rows, b, t,
+                  hq, hk)
     return yq
 
 
@@ -461,11 +474,10 @@ def kv4_read(pages, page_table, row_start, ctx_len, rows):
     whole sequences, pass row_start with ctx_len's running sums."""
     place, where, b = _kv4_place(pages, page_table, row_start, ctx_len)
     hk = pages.shape[1]
-    with torch.cuda.device(pages.device):
-        k = torch.empty((hk, rows, 128), device=pages.device, dtype=BF16)
-        v = torch.empty_like(k)
-        if rows:
-            call("ffb_kv4_read", *place, *where, ptr(k), ptr(v), b, int(rows), hk, stream_ptr())
+    k = torch.empty((hk, rows, 128), device=pages.device, dtype=BF16)
+    v = torch.empty_like(k)
+    if rows:
+        _kv4_call(pages.device, "ffb_kv4_read", *place, *where, k.data_ptr(), v.data_ptr(), b, rows, hk)
     return k, v
 
 
@@ -479,19 +491,15 @@ def attention_kv4(q, pages, page_table, row_start, ctx_len, scale, window=0, sin
     place, where, b = _kv4_place(pages, page_table, row_start, ctx_len)
     _bf16_cuda(q)
     _need(q.dim() == 3 and q.shape[2] == 128 and q.is_contiguous(), "q must be contiguous [HQ, T, 128]")
-    hq, t, _ = q.shape
-    hk = pages.shape[1]
-    _need(hq > 0 and hq % hk == 0, f"{hq} query heads for {hk} K/V heads")
-    _need(q.device == pages.device, "tensors on one device")
-    most = t if max_rows is None else min(int(max_rows), t)
-    _need(most > 0 or t == 0, f"max_rows {max_rows}")
-    with torch.cuda.device(q.device):
-        y = torch.empty((t, hq, 128), device=q.device, dtype=BF16) if out is None else out
-        _need(y.shape == (t, hq, 128) and y.dtype == BF16 and y.is_contiguous() and y.device == q.device,
-              f"out must be contiguous bf16 [{t}, {hq}, 128]")
-        if t:
-            need = L.lib().ffb_attention_kv4_workspace(b, t, hq, hk, most, page_table.shape[1], int(window), int(sinks))
-            ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-            call("ffb_attention_kv4", ptr(q), *place, *where, ptr(y), ptr(ws), need, b, t, most, hq, hk, float(scale),
-                 int(window), int(sinks), stream_ptr())
+    (hq, t, _), hk, dev = q.shape, pages.shape[1], pages.device
+    _need(hq > 0 and hq % hk == 0, "query heads must be a multiple of the K/V heads")
+    _need(q.device == dev, "tensors on one device")
+    most = t if max_rows is None else min(max_rows, t)
+    _need(most > 0 or t == 0, "max_rows must be positive")
+    y = _kv4_out(out, (t, hq, 128), dev)
+    if t:
+        need = L.lib().ffb_attention_kv4_workspace(b, t, hq, hk, most, place[4], window, sinks)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        _kv4_call(dev, "ffb_attention_kv4", q.data_ptr(), *place, *where, y.data_ptr(), ws.data_ptr() if need else None,
+                  need, b, t, most, hq, hk, scale, window, sinks)
     return y
