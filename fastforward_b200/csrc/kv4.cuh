@@ -63,8 +63,10 @@ __device__ __forceinline__ uint8_t* record_of(const Seqs& s, int b, int64_t pos,
 struct AttnArgs {
   const uint16_t* q;  // [HQ, T, 128]
   uint16_t* out;      // [T, HQ, 128]
-  float* part_o;      // [splits][T * HQ][128], relative to part_ml's maximum (splits > 1)
-  float* part_ml;     // [splits][T * HQ][2]
+  uint64_t* flags;    // [CTAs][2]: `tag` once that part is written (register path, equal runs)
+  uint64_t tag;
+  float* part_o;      // partial rows of 128, relative to their maxima: register path [CTAs][2][columns], TC [splits][T * HQ]
+  float* part_ml;     // their (maximum, sum) pairs
   Seqs seqs;
   int HQ, splits, window, sinks;
   float scale_log2;

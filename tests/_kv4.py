@@ -152,10 +152,10 @@ def attention(q, pages, table, starts, lens, scale, window, sinks):
     """o [T, HQ, 128] fp64 and how far a kernel may be off:
       - a probability (times V's scale) is rounded to bf16: 2^-8 of its term; exp2's
         approximation, the fp32 sums and the scale's product stay below 2^-15 of it;
-      - K's codes are multiplied with an offset, |code + 136| <= 143, that the accumulator starts
-        without: its fp32 steps (two MMAs of 16 products and the start, at most 2^-23 of the
-        largest partial sum each, 2^-21 in all) move a score by at most
-        2^-21 143 sum_group s_group sum|q|, a probability by that times |scale|, o by twice that;
+      - K's codes may be multiplied with an offset, code + 8 <= 15, whose 8 sum(q) is taken off
+        afterwards: the fp32 steps (two MMAs of 16 products and the subtraction, at most 2^-23 of
+        the largest partial sum each, 2^-21 in all) move a score by at most
+        2^-21 23 sum_group s_group sum|q|, a probability by that times |scale|, o by twice that;
       - the result is rounded to bf16: 2^-8 of itself."""
     hq, total, _ = q.shape
     hk = pages.shape[1]
@@ -180,6 +180,6 @@ def attention(q, pages, table, starts, lens, scale, window, sinks):
         top = pages[table[b, :-(-n // 64)].long()][..., 8192:8704].contiguous().view(torch.bfloat16).double()
         top = top.reshape(-1, hk, 64, 4).transpose(0, 1).reshape(hk, -1, 4)[:, :n].amax(1).repeat_interleave(hq // hk, 0)
         mass = (q[:, r0:r1].double().abs().reshape(hq, -1, 4, 32).sum(-1) * top[:, None]).sum(-1).T[..., None]
-        shift = 2 * abs(scale) * 2.0 ** -21 * 143 * mass
+        shift = 2 * abs(scale) * 2.0 ** -21 * 23 * mass
         limit[r0:r1] += spread * (2.0 ** -8 + 2.0 ** -15) * 1.01 + (spread + out[r0:r1].abs()) * shift + out[r0:r1].abs() * 2.0 ** -8 * 1.01
     return out, limit

@@ -178,6 +178,18 @@ def test_long_chunks_with_a_small_hint(rows, ctx):
     _attend(rows, ctx, 8, 2, seed=32, max_rows=5, window=70, sinks=5)
 
 
+@pytest.mark.parametrize("seed", range(4))
+def test_ragged_batches_share_the_pages(seed):
+    """Lengths from nothing to many pages: the runs of pages that the CTAs take cut items anywhere,
+    hold many short ones whole, and skip sequences without rows."""
+    g = torch.Generator().manual_seed(seed)
+    b = [3, 40, 300, 17][seed]
+    ctx = [int(x) for x in (torch.rand(b, generator=g) ** 4 * [6000, 1500, 150, 3000][seed]).long()]
+    rows = [int(x) for x in torch.randint(0, 3, (b,), generator=g)]
+    rows[0] = 1
+    _attend(rows, ctx, [8, 8, 2, 24][seed], [2, 1, 1, 2][seed], seed=seed, max_rows=2, lead=1, tail=1)
+
+
 def test_rows_that_see_nothing_are_zero():
     """More rows than the sequence holds: the first of them lie before its start."""
     got = _attend([4, 2], [1, 0], 4, 2, seed=2, max_rows=4)
@@ -188,6 +200,52 @@ def test_rows_that_see_nothing_are_zero():
 def test_scales(scale):
     """scale 30 gives scores of thousands: the running maximum has to carry them."""
     _attend([1, 6], [333, 70], 8, 2, seed=4, scale=scale, max_rows=6)
+
+
+def test_queries_of_any_size():
+    """Columns from tiny to huge next to each other, with elements far below their column's largest:
+    queries are scaled per column for the tensor core."""
+    hk, hq = 1, 8
+    g = torch.Generator().manual_seed(0)
+    pages = ref.pack(*(torch.randn(5, hk, 64, 128, generator=g, dtype=torch.float64) for _ in range(2)))
+    q = torch.randn(hq, 1, 128, generator=g) * torch.logspace(-30, 6, hq)[:, None, None]
+    q[:, :, ::3] *= 2.0 ** -20
+    q[3] = 0
+    q = q.to(BF16)
+    table = torch.arange(5, dtype=torch.int32)[None]
+    starts, lens = torch.tensor([0, 1], dtype=torch.int32), torch.tensor([300], dtype=torch.int32)
+    got = ops.attention_kv4(_dev(q), _dev(pages), _dev(table), _dev(starts), _dev(lens), 0.05).cpu()
+    want, limit = ref.attention(q, pages, table, starts, lens, 0.05, 0, 0)
+    assert ((got.double() - want).abs() <= limit).all()
+
+
+@pytest.mark.parametrize("rows", [1, 3, 40])
+def test_nan_reaches_only_the_rows_that_see_it(rows):
+    """A key or value that reads as NaN: rows that see it are NaN (the whole row, or the value's
+    scale group), rows before it or past the window are exact."""
+    hk, hq, n = 1, 4, 200
+    g = torch.Generator().manual_seed(0)
+    k, v = (torch.randn(4, hk, 64, 128, generator=g, dtype=torch.float64) for _ in range(2))
+    clean = ref.pack(k, v)
+    table = torch.arange(4, dtype=torch.int32)[None]
+    q = torch.randn(hq, rows, 128, generator=g).to(BF16)
+    starts, lens = torch.tensor([0, rows], dtype=torch.int32), torch.tensor([n], dtype=torch.int32)
+    at = n - 1 - rows // 2  # seen by the last rows only
+    for base in (8192, 8704):
+        pages = clean.clone()
+        sc = pages[at // 64, 0, base + 8 * (at % 64):base + 8 * (at % 64) + 2]
+        sc.copy_(torch.tensor([0xC0, 0x7F], dtype=torch.uint8))
+        got = ops.attention_kv4(_dev(q), _dev(pages), _dev(table), _dev(starts), _dev(lens), 0.1, max_rows=rows).cpu()
+        want, limit = ref.attention(q, clean, table, starts, lens, 0.1, 0, 0)
+        before = rows - 1 - rows // 2  # rows whose position lies before `at`
+        assert ((got.double() - want).abs() <= limit)[:before].all()
+        assert got[before:, :, :32].isnan().all()
+        got = ops.attention_kv4(_dev(q), _dev(pages), _dev(table), _dev(starts), _dev(lens), 0.1, max_rows=rows,
+                                window=max(1, rows // 2)).cpu()
+        want, limit = ref.attention(q, clean, table, starts, lens, 0.1, max(1, rows // 2), 0)
+        far = torch.arange(n - rows, n) - at  # distance of each row's position from the poisoned key
+        free = (far < 0) | (far >= max(1, rows // 2))
+        assert ((got.double() - want).abs() <= limit)[free].all() and got[~free][:, :, :32].isnan().all()
 
 
 def test_growing_scores_move_the_maximum():

@@ -71,8 +71,9 @@ def test_workspace_is_zero_for_bad_shapes_and_bounded():
     assert f(0, 1, 4, 1, 1, 1, 0, 0) == 0 and f(1, 1, 3, 2, 1, 1, 0, 0) == 0
     assert f(1, 1, 32, 8, 1, 1, 0, 0) == 0  # one page is not shared out
     many = f(1, 1, 32, 8, 1, 4096, 0, 0)
-    assert 0 < many <= 64 * 32 * 130 * 4
-    assert f(1, 1, 32, 8, 1, 4096, 64, 0) < many  # a window bounds the pages
+    assert 0 < many <= 8 << 20 and many == f(1, 1, 32, 8, 1, 1 << 24, 0, 0)  # the context's length does not count
+    assert f(1, 1, 32, 8, 1, 4096, 64, 0) == 0  # a window bounds the pages
+    assert 0 < f(1, 64, 32, 8, 64, 4096, 0, 0) <= 64 * 64 * 32 * 130 * 4
 
 
 def test_python_calls_refuse_cpu_tensors():
