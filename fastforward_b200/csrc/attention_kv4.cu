@@ -183,6 +183,29 @@ __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;
 __device__ __forceinline__ void st_release_gpu_u64(uint64_t* p, uint64_t v) {
   asm volatile("st.release.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(v) : "memory");
 }
+// mbarrier and bulk copy on shared-memory addresses held as integers.
+__device__ __forceinline__ void expect_bytes(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool arrived(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ void bulk(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
 // The token of fragment row r (0..7): 2 <-> 3 and 6 <-> 7 trade places, so that the eight lanes
 // of a load phase meet rows of both parities and, with V's exchanged halves, all banks.
 __device__ __forceinline__ int token_of(int r) { return r ^ ((r >> 1) & 1); }
@@ -205,6 +228,12 @@ __device__ __forceinline__ void add_part(Sum& s, float m, float l, float4 v) {
 __device__ __forceinline__ void store_row(uint16_t* out, const Sum& s, int lane) {
   const float r = s.l == 0.f ? 0.f : 1.f / s.l;
   *reinterpret_cast<uint2*>(out + 4 * lane) = make_uint2(pack_bf16(s.o.x * r, s.o.y * r), pack_bf16(s.o.z * r, s.o.w * r));
+}
+
+// a b / c, in 32 bits where that is enough (a 64-bit division takes hundreds of cycles).
+__device__ __forceinline__ int64_t mul_div(int a, int64_t b, int c) {
+  if (b < (1 << 22) && a < 1024) return (uint32_t)a * (uint32_t)b / (uint32_t)c;
+  return a * b / c;
 }
 
 template <int NT, bool WHOLE>
@@ -267,8 +296,8 @@ __global__ void __launch_bounds__(THREADS, Shape<NT>::PER_SM) kv4_attention_kern
     }
     sharing = (int)max((int64_t)1, min((int64_t)gridDim.x, total / MIN_PAGES));
     if ((int)blockIdx.x >= sharing) return;
-    at = blockIdx.x * total / sharing;
-    const int64_t end = (blockIdx.x + 1) * total / sharing;
+    at = mul_div(blockIdx.x, total, sharing);
+    const int64_t end = mul_div(blockIdx.x + 1, total, sharing);
     if (at >= end) return;  // no rows at all
     if (at >= pre && at < pre + mine) {
       int i = b_lo;
@@ -280,8 +309,8 @@ __global__ void __launch_bounds__(THREADS, Shape<NT>::PER_SM) kv4_attention_kern
           const int span = ITEM_PAGES + seq.pages();
           run.left = end - at;
           run.b = i;
-          run.item = (int)((at - p) / span);
-          run.from = (int)((at - p) % span) - ITEM_PAGES;
+          run.item = (int)(at - p < 0x7fffffff ? (uint32_t)(at - p) / (uint32_t)span : (at - p) / span);
+          run.from = (int)(at - p - (int64_t)run.item * span) - ITEM_PAGES;
           break;
         }
         p += w;
@@ -349,9 +378,8 @@ __global__ void __launch_bounds__(THREADS, Shape<NT>::PER_SM) kv4_attention_kern
   // the ring is full and `use` is done with).  Bit s of `bad`: the page of stage s is outside the cache.
   int use = 0, fill = 0;
   uint32_t use_ph = 0, bad = 0;
-  uint64_t* wfull = full + warp * STAGES;
-  uint8_t* wring = smem + warp * STAGES * HALF_BYTES;
-  const int64_t head_stride = (int64_t)sv.HK * RECORD;
+  const uint32_t wfull = smem_u32(full + warp * STAGES), wring = smem_u32(smem + warp * STAGES * HALF_BYTES);
+  const uint32_t page_bytes = (uint32_t)sv.HK * RECORD;
   // pages i0 + group + GROUPS k of a share are this warp's
   auto pages_in = [&](const Share& s) { return max(0, (s.i1 - s.i0 - group + GROUPS - 1) / GROUPS); };
   auto page_index = [&](const PageSet& ps, int i) { return i < ps.n_sink ? i : ps.first_page + i - ps.n_sink; };
@@ -359,27 +387,26 @@ __global__ void __launch_bounds__(THREADS, Shape<NT>::PER_SM) kv4_attention_kern
   auto ids_from = [&](const Share& s, int k, int cnt) {
     return k + lane < cnt ? __ldg(sv.table + s.b * sv.table_stride + page_index(s.ps, s.i0 + group + GROUPS * (k + lane))) : -1;
   };
-  auto load = [&](int page, int kvh) {  // the whole warp
-    const int stage = fill;
-    fill = fill + 1 == STAGES ? 0 : fill + 1;
-    if (page >= 0 && page < sv.num_pages) {
-      bad &= ~(1u << stage);
+  auto load = [&](int page, const uint8_t* head) {  // the whole warp; head: page 0's record of the K/V head
+    const uint32_t bar = wfull + 8 * fill, dst = wring + HALF_BYTES * fill;
+    if ((uint32_t)page < (uint32_t)sv.num_pages) {
       if (lane == 0) {
-        const uint8_t* src = sv.pages + page * head_stride + kvh * RECORD;
-        uint8_t* dst = wring + stage * HALF_BYTES;
-        mbar_arrive_expect_tx(&wfull[stage], HALF_BYTES);
-        bulk_load(dst, src + 64 * tok0, HALF_CODES, &wfull[stage]);
-        bulk_load(dst + HALF_KS, src + K_SCALES + 8 * tok0, HALF_SCALES, &wfull[stage]);
-        bulk_load(dst + HALF_V, src + V_CODES + 64 * tok0, HALF_CODES, &wfull[stage]);
-        bulk_load(dst + HALF_VS, src + V_SCALES + 8 * tok0, HALF_SCALES, &wfull[stage]);
+        const uint8_t* codes = head + (uint64_t)(uint32_t)page * page_bytes + 64 * tok0;
+        const uint8_t* scales = codes - 56 * tok0;
+        expect_bytes(bar, HALF_BYTES);
+        bulk(dst, codes, HALF_CODES, bar);
+        bulk(dst + HALF_KS, scales + K_SCALES, HALF_SCALES, bar);
+        bulk(dst + HALF_V, codes + V_CODES, HALF_CODES, bar);
+        bulk(dst + HALF_VS, scales + V_SCALES, HALF_SCALES, bar);
       }
     } else {
-      bad |= 1u << stage;
+      bad |= 1u << fill;
       if (lane == 0) {
         atomicOr(&ffb_device_error_word, (uint32_t)ffb::ERR_KV4_PAGE);
-        mbar_arrive(&wfull[stage]);
+        arrive(bar);
       }
     }
+    fill = fill + 1 == STAGES ? 0 : fill + 1;
   };
   // where this lane reads in a half page: K codes of token token_of(g), scales, V codes of the
   // tokens of MMA columns 2 t and 2 t + 1
@@ -414,7 +441,8 @@ __global__ void __launch_bounds__(THREADS, Shape<NT>::PER_SM) kv4_attention_kern
     const int cnt = pages_in(first);
     ids = ids_from(first, 0, cnt);
     fetch_queries(first, 0);
-    for (; issued < min(cnt, STAGES); ++issued) load(__shfl_sync(0xffffffffu, ids, issued), first.kvh);
+    const uint8_t* head = sv.pages + (int64_t)first.kvh * RECORD;
+    for (; issued < min(cnt, STAGES); ++issued) load(__shfl_sync(0xffffffffu, ids, issued), head);
   }
   while (more) {
     const Share& cur = run.share[turn];
@@ -461,16 +489,18 @@ __global__ void __launch_bounds__(THREADS, Shape<NT>::PER_SM) kv4_attention_kern
 
     // the ids of the next share's first pages, for the stages that this one's last pages leave, and its queries
     more = run.more;
-    int next_cnt = 0, next_ids = -1, next_kvh = 0, ahead = 0;
+    int next_cnt = 0, next_ids = -1, ahead = 0;
+    const uint8_t* next_head = sv.pages;
     if (more) {
       const Share& next = run.share[turn ^ 1];
-      next_kvh = next.kvh;
+      next_head += (int64_t)next.kvh * RECORD;
       next_cnt = pages_in(next);
       next_ids = ids_from(next, 0, next_cnt);
       fetch_queries(next, turn ^ 1);
     }
     const PageSet ps = cur.ps;
-    const int i0 = cur.i0, kvh = cur.kvh, whole_lo = cur.whole_lo, whole_hi = cur.whole_hi, cnt = pages_in(cur);
+    const int i0 = cur.i0, whole_lo = cur.whole_lo, whole_hi = cur.whole_hi, cnt = pages_in(cur);
+    const uint8_t* head = sv.pages + (int64_t)cur.kvh * RECORD;
     uint2 qo[NT];  // K index 4 part + j of the offsets' MMA: this lane has 2 t, 2 t + 1 and 8 more (part 3: zeros)
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -642,16 +672,19 @@ __global__ void __launch_bounds__(THREADS, Shape<NT>::PER_SM) kv4_attention_kern
     bool ok = true;
     for (int k = 0; k < cnt; ++k) {
       // one verdict for the warp: its lanes stay together whatever each of them saw
-      if (!__all_sync(0xffffffffu, mbar_try_wait(&wfull[use], use_ph)) &&
-          !__all_sync(0xffffffffu, mbar_wait_bounded(&wfull[use], use_ph, abort_flag))) {
+      if (!__all_sync(0xffffffffu, arrived(wfull + 8 * use, use_ph)) &&
+          !__all_sync(0xffffffffu, mbar_wait_bounded(full + warp * STAGES + use, use_ph, abort_flag))) {
         ok = false;
         break;
       }
-      const int i = i0 + group + GROUPS * k;
       if (!((bad >> use) & 1u)) {
-        const uint8_t* rec = wring + use * HALF_BYTES;
-        const int key0 = page_index(ps, i) * PAGE + tok0;
-        if (key0 < ps.kend) tokens(rec, key0, i < whole_lo || i >= whole_hi);
+        const int i = i0 + group + GROUPS * k;
+        const bool masked = i < whole_lo || i >= whole_hi;
+        int key0 = 0;
+        if (masked) key0 = page_index(ps, i) * PAGE + tok0;
+        if (!masked || key0 < ps.kend) tokens(smem + (warp * STAGES + use) * HALF_BYTES, key0, masked);
+      } else {
+        bad &= ~(1u << use);
       }
       __syncwarp();  // every lane has read the stage
       if (issued < cnt) {
@@ -659,10 +692,10 @@ __global__ void __launch_bounds__(THREADS, Shape<NT>::PER_SM) kv4_attention_kern
           ids_at = issued;
           ids = ids_from(cur, ids_at, cnt);
         }
-        load(__shfl_sync(0xffffffffu, ids, issued - ids_at), kvh);
+        load(__shfl_sync(0xffffffffu, ids, issued - ids_at), head);
         ++issued;
       } else if (ahead < next_cnt) {
-        load(__shfl_sync(0xffffffffu, next_ids, ahead), next_kvh);
+        load(__shfl_sync(0xffffffffu, next_ids, ahead), next_head);
         ++ahead;
       }
       if (++use == STAGES) {
@@ -673,15 +706,15 @@ __global__ void __launch_bounds__(THREADS, Shape<NT>::PER_SM) kv4_attention_kern
     if (!ok) *abort_flag = 1;
     // a share with fewer pages than stages leaves some of the ring's to fill
     for (; ahead < min(next_cnt, STAGES) && !*abort_flag; ++ahead)
-      load(__shfl_sync(0xffffffffu, next_ids, ahead), next_kvh);
+      load(__shfl_sync(0xffffffffu, next_ids, ahead), next_head);
     issued = ahead;
     ids = next_ids;
     ids_at = 0;
     if (lane == 0 && *abort_flag) {  // copies in flight must land before the CTA leaves
       volatile int never = 0;
       for (int i = 0; i < STAGES; ++i) {
-        mbar_wait_bounded(&wfull[i], 0, &never, 20000000ull);
-        mbar_wait_bounded(&wfull[i], 1, &never, 20000000ull);
+        mbar_wait_bounded(full + warp * STAGES + i, 0, &never, 20000000ull);
+        mbar_wait_bounded(full + warp * STAGES + i, 1, &never, 20000000ull);
       }
     }
 #pragma unroll
@@ -729,7 +762,7 @@ __global__ void __launch_bounds__(THREADS, Shape<NT>::PER_SM) kv4_attention_kern
           y.z = fmaf(v.z, f, y.z);
           y.w = fmaf(v.w, f, y.w);
         }
-        const int row = cur.r0 + col / G, h = kvh * G + col % G;
+        const int row = cur.r0 + col / G, h = cur.kvh * G + col % G;
         if (cur.entire) {
           const float r = sum == 0.f ? 0.f : 1.f / sum;  // nothing visible: zeros
           *reinterpret_cast<uint2*>(args.out + ((int64_t)row * args.HQ + h) * D + d) =
