@@ -481,8 +481,9 @@ __global__ void __launch_bounds__(THREADS, Shape<NT>::PER_SM) kv4_attention_kern
       if (t == 0) {
         ssum[(8 * n + g) * 4 + j] = sum * -0x1p-21f;  // -8 x 2^-24
         // scores come out 2^-24 factor times too large; beyond 2^110 the (one-hot) softmax only
-        // needs their order
-        if (j == 0) smul[8 * n + g] = fabsf(args.scale_log2) * __uint_as_float((uint32_t)(127 + 10 + min(ex, 110)) << 23);
+        // needs their order.  Never 0: a masked -inf stays one
+        if (j == 0)
+          smul[8 * n + g] = fmaxf(fabsf(args.scale_log2) * __uint_as_float((uint32_t)(127 + 10 + min(ex, 110)) << 23), 1e-37f);
       }
     }
     __syncthreads();

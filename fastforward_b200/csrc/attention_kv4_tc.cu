@@ -69,6 +69,25 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// fp32 pairs in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 u, v, w;\n\t"
+      "mov.b64 u, {%2, %3};\n\tmov.b64 v, {%4, %5};\n\tmov.b64 w, {%6, %7};\n\t"
+      "fma.rn.f32x2 u, u, v, w;\n\tmov.b64 {%0, %1}, u;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 u, v;\n\t"
+      "mov.b64 u, {%2, %3};\n\tmov.b64 v, {%4, %5};\n\t"
+      "add.rn.f32x2 u, u, v;\n\tmov.b64 {%0, %1}, u;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
 __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
   const __nv_bfloat162 r =
       __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
@@ -116,6 +135,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(last + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* raw_bad = abort_flag + 1;  // [RAW]: the page is absent or its id outside the cache
+  // [16] the same of the pages of block u, two bits: what the softmax of that block masks.  It follows
+  // the producer through the pages' and tiles' barriers by at most eight blocks.
+  volatile int* blk_bad = raw_bad + RAW;
 
   const Seqs& sv = args.seqs;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -180,6 +202,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
     if (warp == 0) {
       // ---------------------------------------------------------------- raw pages
       if (lane == 0) {
+        int bad_pair = 0;
         for (int i = 0; i < 2 * nblk; ++i) {
           const uint32_t u = 2 * blk0 + i, s = u % RAW;
           if (u >= RAW && !mbar_wait_bounded(&raw_empty[s], ((u / RAW) & 1u) ^ 1u, abort_flag)) {
@@ -195,6 +218,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
             }
           }
           raw_bad[s] = page < 0;
+          bad_pair = (i & 1) ? bad_pair | (page < 0 ? 2 : 0) : (page < 0 ? 1 : 0);
+          if (i & 1) blk_bad[(blk0 + (i >> 1)) & 15] = bad_pair;
           if (page >= 0) {
             mbar_arrive_expect_tx(&raw_full[s], RECORD);
             bulk_load(raw + s * RECORD, sv.pages + ((int64_t)page * sv.HK + kvh) * RECORD, RECORD, &raw_full[s]);
@@ -364,7 +389,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
         const bool live_row = col <= clast;
         const int row = live_row ? r0 + col / G : 0, head = live_row ? kvh * G + col % G : 0;
         const int pos = live_row ? ctx - S + col / G : -1;
-        const float sc = fabsf(args.scale_log2);
+        const float sc = fmaxf(fabsf(args.scale_log2), 1e-37f);  // scale 0: a masked -inf stays one
         // this warp's 32 rows of Q, negated for a negative scale (exact), eight channels a chunk in
         // the order 0 4 1 5 2 6 3 7; sixteen lanes copy one row.  A tile without blocks has no queries:
         // no product would keep its warps from staging output over rows that others still write
@@ -388,53 +413,62 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
         }
         const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
         const uint32_t st = tmem + lane_addr + 128 * x, ot = tmem + lane_addr + 256 + 128 * x;
-        float m = -INFINITY, l = 0.f;
+        float m = -INFINITY, neg = 0.f, l = 0.f;  // neg: -m, 0 while nothing has been seen
+        const float2 sc2 = make_float2(sc, sc);
         for (int j = 0; j < nblk; ++j) {
           if (!__all_sync(0xffffffffu, mbar_wait_bounded(&s_full[x], (base_blk + j) & 1u, abort_flag) && !*abort_flag)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const int ia = i0 + 2 * j;
-          const bool has_b = ia + 1 < i1;
-          const int ka = page_index(ia) * PAGE, kb = has_b ? page_index(ia + 1) * PAGE : ps.kend;
+          const int ia = i0 + 2 * j, bad = blk_bad[(blk0 + j) & 15];
+          const int ka = page_index(ia) * PAGE, kb = page_index(ia + 1) * PAGE;
           auto seen_by_all = [&](int key0) {
             return key0 + PAGE - 1 <= pos_lo && key0 + PAGE <= ps.kend &&
                    (args.window == 0 || pos_hi - key0 < args.window || key0 + PAGE <= args.sinks);
           };
-          const int pa = __ldg(table + page_index(ia)), pb = has_b ? __ldg(table + page_index(ia + 1)) : -1;
-          const bool good_a = pa >= 0 && pa < sv.num_pages, good_b = pb >= 0 && pb < sv.num_pages;
-          const bool whole = has_b && good_a && good_b && seen_by_all(ka) && seen_by_all(kb);
+          const bool whole = bad == 0 && seen_by_all(ka) && seen_by_all(kb);
           // columns of this row that count, per page: c <= hi and (c >= lo or c < sk)
           const int top = min(pos, ps.kend - 1), low = args.window > 0 ? pos - args.window + 1 : 0;
-          const int hi[2] = {good_a ? top - ka : -1, good_b ? top - kb : -1};
+          const int hi[2] = {(bad & 1) ? -1 : top - ka, (bad & 2) ? -1 : top - kb};
           const int lo[2] = {low - ka, low - kb}, sk[2] = {args.sinks - ka, args.sinks - kb};
-          float bmax = -INFINITY;
+          // the largest score, a quarter of the row ahead of what is compared
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          uint32_t v[2][32];
+          tmem_ld32_async(st, v[0]);
+          if (whole) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t v[32];
-            tmem_ld32_async(st + 32 * q, v);
-            tmem_wait_ld();
-            reg_fence(v);
-            if (whole) {
+            for (int q = 0; q < 4; ++q) {
+              tmem_wait_ld();
+              reg_fence(v[q & 1]);
+              if (q < 3) tmem_ld32_async(st + 32 * (q + 1), v[(q + 1) & 1]);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) bmax = fmaxf(bmax, __uint_as_float(v[e]));
-            } else {
+              for (int e = 0; e < 32; e += 2)
+                mx[(e >> 1) & 3] = fmaxf(mx[(e >> 1) & 3], fmaxf(__uint_as_float(v[q & 1][e]), __uint_as_float(v[q & 1][e + 1])));
+            }
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              tmem_wait_ld();
+              reg_fence(v[q & 1]);
+              if (q < 3) tmem_ld32_async(st + 32 * (q + 1), v[(q + 1) & 1]);
 #pragma unroll
               for (int e = 0; e < 32; ++e) {
                 const int c = 32 * (q & 1) + e;
-                if (c <= hi[q >> 1] && (c >= lo[q >> 1] || c < sk[q >> 1])) bmax = fmaxf(bmax, __uint_as_float(v[e]));
+                if (c <= hi[q >> 1] && (c >= lo[q >> 1] || c < sk[q >> 1])) mx[0] = fmaxf(mx[0], __uint_as_float(v[q & 1][e]));
               }
             }
           }
-          bmax *= sc;
-          if (!(bmax > -INFINITY)) bmax = -INFINITY;  // scale 0 of an empty row: 0 x -inf
+          tmem_ld32_async(st, v[0]);  // again, for the probabilities
+          float bmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          bmax = bmax == -INFINITY ? bmax : bmax * sc;
           const bool grow = bmax > m + LAZY;
           if (__any_sync(0xffffffffu, grow)) {
             const float nm = grow ? bmax : m;
             const float alpha = grow ? ex2(m - nm) : 1.f;
             l *= alpha;
             m = nm;
+            neg = m == -INFINITY ? 0.f : -m;
             if (j > 0) {
               if (!__all_sync(0xffffffffu, mbar_wait_bounded(&o_done[x], (base_blk + j - 1) & 1u, abort_flag))) {
                 ok = false;
@@ -443,40 +477,42 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
               tc_fence_after();
 #pragma unroll 1
               for (int q = 0; q < 8; ++q) {
-                uint32_t v[16];
-                tmem_ld16_async(ot + 16 * q, v);
+                uint32_t w[16];
+                tmem_ld16_async(ot + 16 * q, w);
                 tmem_wait_ld();
-                reg_fence(v);
+                reg_fence(w);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * alpha);
-                tmem_st16(ot + 16 * q, v);
+                for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(__uint_as_float(w[e]) * alpha);
+                tmem_st16(ot + 16 * q, w);
               }
               tmem_wait_st();
             }
           }
-          const float neg = m == -INFINITY ? 0.f : -m;
-          float sum[2] = {0.f, 0.f};
+          const float2 neg2 = make_float2(neg, neg);
+          float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            uint32_t v[32], p[16];
-            tmem_ld32_async(st + 32 * q, v);
+            uint32_t p[16];
             tmem_wait_ld();
-            reg_fence(v);
+            reg_fence(v[q & 1]);
+            if (q < 3) tmem_ld32_async(st + 32 * (q + 1), v[(q + 1) & 1]);
+            if (!whole) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) {
+                const int c = 32 * (q & 1) + e;
+                if (!(c <= hi[q >> 1] && (c >= lo[q >> 1] || c < sk[q >> 1]))) v[q & 1][e] = 0xff800000u;  // -inf
+              }
+            }
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
-              float y0 = ex2(fmaf(__uint_as_float(v[e]), sc, neg)), y1 = ex2(fmaf(__uint_as_float(v[e + 1]), sc, neg));
-              if (!whole) {
-                const int c = 32 * (q & 1) + e, h = q >> 1;
-                if (!(c <= hi[h] && (c >= lo[h] || c < sk[h]))) y0 = 0.f;
-                if (!(c + 1 <= hi[h] && (c + 1 >= lo[h] || c + 1 < sk[h]))) y1 = 0.f;
-              }
-              sum[0] += y0;
-              sum[1] += y1;
-              p[e >> 1] = pack_bf16(y0, y1);
+              const float2 y = fma2(make_float2(__uint_as_float(v[q & 1][e]), __uint_as_float(v[q & 1][e + 1])), sc2, neg2);
+              const float2 z = make_float2(ex2(y.x), ex2(y.y));
+              sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], z);
+              p[e >> 1] = pack_bf16(z.x, z.y);
             }
             tmem_st16(st + 16 * q, p);
           }
-          l += sum[0] + sum[1];
+          l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();

@@ -200,6 +200,8 @@ def test_rows_that_see_nothing_are_zero():
 def test_scales(scale):
     """scale 30 gives scores of thousands: the running maximum has to carry them."""
     _attend([1, 6], [333, 70], 8, 2, seed=4, scale=scale, max_rows=6)
+    _attend([1, 1, 1], [333, 70, 1], 8, 2, seed=5, scale=scale, max_rows=1)
+    _attend([1, 2], [900, 2], 16, 2, seed=6, scale=scale, max_rows=2, window=100, sinks=1)
 
 
 def test_queries_of_any_size():
