@@ -888,23 +888,23 @@ struct Plan {
 
 // TC's shares: enough CTAs for every SM, against the start and end of a CTA and the join.
 // step_us, cta_us: what a block of two pages and a CTA's start and end take; join_us: a share's
-// partials, written and read.  Only share counts that fill whole waves are compared.
+// partials, written and read.
 int plan_splits(int64_t base, int64_t pages, int slots, double step_us, double cta_us, double join_us) {
   int best = 1;
   double best_cost = 0;
-  for (int wave = 0; wave <= 4; ++wave) {
-    int64_t fit = wave == 0 ? 1 : wave * slots / base;
-    if (fit > pages / 2) fit = pages / 2;
-    const int s = wave == 0 ? 1 : (int)(fit < 64 ? fit : 64);
-    if (s < 1) continue;
+  auto look = [&](int64_t s) {
+    if (s < 1 || s > 64 || (s > 1 && s > pages / 2)) return;
     const double waves = (double)((base * s + slots - 1) / slots);
     const double rounds = (double)((pages + 2 * s - 1) / (2 * s));
     const double cost = waves * (rounds * step_us + cta_us) + (s > 1 ? 2.0 + join_us * s : 0.0);
-    if (wave == 0 || cost < best_cost) {
-      best = s;
+    if (best_cost == 0 || cost < best_cost) {
+      best = (int)s;
       best_cost = cost;
     }
-  }
+  };
+  for (int s = 1; s <= 4; ++s) look(s);
+  for (int wave = 1; wave <= 3; ++wave) look(wave * slots / base);  // whole waves
+  if (slots / base > pages / 2) look(pages / 2);
   return best;
 }
 
@@ -923,7 +923,7 @@ Plan make_plan(int B, int T, int HQ, int HK, int max_rows, int max_pages, int wi
   const int sms = ffb::sm_count();
   if (p.kernel == TC) {
     const double join = (double)T * HQ * (D + 2) * 4 * 2 / 5e6;  // written and read at about 5 TB/s
-    p.splits = plan_splits((int64_t)B * HK * p.tiles, pages, sms, 1.4, 5.0, join);
+    p.splits = plan_splits((int64_t)B * HK * p.tiles, pages, sms, 2.5, 6.0, join);
     p.ctas = B * HK * p.splits;
     p.bytes = p.splits > 1 ? (int64_t)p.splits * T * HQ * (D + 2) * 4 : 0;
   } else {

@@ -9,7 +9,7 @@
 //                S = Q K^T (M 128, N 128, 8 steps of 16 channels), O += P V (8 steps of 16 keys,
 //                P read from tensor memory, V row-major)
 //   warps 4-11   softmax: four warps a tile, one thread a row
-//   warps 12-15  dequantisation: codes and scales of a block -> K and V tiles in bf16 (exact:
+//   warps 12-19  dequantisation: codes and scales of a block -> K and V tiles in bf16 (exact:
 //                five bits times three), 128-byte swizzled, in a ring of three 32 KB slots
 // The dequantisation is paid once per 256 columns, which is what makes the tensor cores worth
 // it over the register path of attention_kv4.cu.  Two query tiles let the MMAs of one run
@@ -30,7 +30,8 @@ namespace {
 
 using namespace kv4;
 
-constexpr int THREADS = 512;
+constexpr int DEQUANT = 8;              // warps
+constexpr int THREADS = 384 + 32 * DEQUANT;
 constexpr int RAW = 6;                 // raw pages in flight
 constexpr int SLOTS = 3;               // 128-key K or V tiles
 constexpr int HALF = 128 * 128;        // 64 channels (K, Q) or columns (V) of 128 rows: 16 KB
@@ -148,10 +149,10 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
   if (tid == 0) {
     for (int i = 0; i < RAW; ++i) {
       mbar_init(&raw_full[i], 1);
-      mbar_init(&raw_empty[i], 4);
+      mbar_init(&raw_empty[i], DEQUANT);
     }
     for (int i = 0; i < SLOTS; ++i) {
-      mbar_init(&slot_full[i], 4);
+      mbar_init(&slot_full[i], DEQUANT);
       mbar_init(&slot_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -319,9 +320,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
             const int key0 = i0 + 2 * j + a < i1 ? page_index(i0 + 2 * j + a) * PAGE : 0;
             // tokens past the newest row's position are held by nobody: whatever is there is not used
             const int live = bad ? 0 : min(max(ps.kend - key0, 0), PAGE);
-#pragma unroll
-            for (int it = 0; it < 2; ++it) {
-              const int r8 = 8 * (w + 4 * it);  // this warp's eight tokens
+            {
+              const int r8 = 8 * w;  // this warp's eight tokens
               if (!is_v) {
                 // token pairs (r, r ^ 5) x four chunks meet all banks on the load and on the store
                 const int k = lane >> 3, e = (lane >> 2) & 1, t = lane & 3;
@@ -432,34 +432,25 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
           const int top = min(pos, ps.kend - 1), low = args.window > 0 ? pos - args.window + 1 : 0;
           const int hi[2] = {(bad & 1) ? -1 : top - ka, (bad & 2) ? -1 : top - kb};
           const int lo[2] = {low - ka, low - kb}, sk[2] = {args.sinks - ka, args.sinks - kb};
-          // the largest score, a quarter of the row ahead of what is compared
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          uint32_t v[2][32];
-          tmem_ld32_async(st, v[0]);
-          if (whole) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              tmem_wait_ld();
-              reg_fence(v[q & 1]);
-              if (q < 3) tmem_ld32_async(st + 32 * (q + 1), v[(q + 1) & 1]);
+          for (int q = 0; q < 4; ++q) {
+            uint32_t v[32];
+            tmem_ld32_async(st + 32 * q, v);
+            tmem_wait_ld();
+            reg_fence(v);
+            if (whole) {
 #pragma unroll
               for (int e = 0; e < 32; e += 2)
-                mx[(e >> 1) & 3] = fmaxf(mx[(e >> 1) & 3], fmaxf(__uint_as_float(v[q & 1][e]), __uint_as_float(v[q & 1][e + 1])));
-            }
-          } else {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              tmem_wait_ld();
-              reg_fence(v[q & 1]);
-              if (q < 3) tmem_ld32_async(st + 32 * (q + 1), v[(q + 1) & 1]);
+                mx[(e >> 1) & 3] = fmaxf(mx[(e >> 1) & 3], fmaxf(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
+            } else {
 #pragma unroll
               for (int e = 0; e < 32; ++e) {
                 const int c = 32 * (q & 1) + e;
-                if (c <= hi[q >> 1] && (c >= lo[q >> 1] || c < sk[q >> 1])) mx[0] = fmaxf(mx[0], __uint_as_float(v[q & 1][e]));
+                if (c <= hi[q >> 1] && (c >= lo[q >> 1] || c < sk[q >> 1])) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(v[e]));
               }
             }
           }
-          tmem_ld32_async(st, v[0]);  // again, for the probabilities
           float bmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
           bmax = bmax == -INFINITY ? bmax : bmax * sc;
           const bool grow = bmax > m + LAZY;
@@ -492,20 +483,20 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
           float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            uint32_t p[16];
+            uint32_t v[32], p[16];
+            tmem_ld32_async(st + 32 * q, v);
             tmem_wait_ld();
-            reg_fence(v[q & 1]);
-            if (q < 3) tmem_ld32_async(st + 32 * (q + 1), v[(q + 1) & 1]);
+            reg_fence(v);
             if (!whole) {
 #pragma unroll
               for (int e = 0; e < 32; ++e) {
                 const int c = 32 * (q & 1) + e;
-                if (!(c <= hi[q >> 1] && (c >= lo[q >> 1] || c < sk[q >> 1]))) v[q & 1][e] = 0xff800000u;  // -inf
+                if (!(c <= hi[q >> 1] && (c >= lo[q >> 1] || c < sk[q >> 1]))) v[e] = 0xff800000u;  // -inf
               }
             }
 #pragma unroll
             for (int e = 0; e < 32; e += 2) {
-              const float2 y = fma2(make_float2(__uint_as_float(v[q & 1][e]), __uint_as_float(v[q & 1][e + 1])), sc2, neg2);
+              const float2 y = fma2(make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), sc2, neg2);
               const float2 z = make_float2(ex2(y.x), ex2(y.y));
               sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], z);
               p[e >> 1] = pack_bf16(z.x, z.y);
