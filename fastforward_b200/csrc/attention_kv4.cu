@@ -893,7 +893,7 @@ int plan_splits(int64_t base, int64_t pages, int slots, double step_us, double c
   int best = 1;
   double best_cost = 0;
   auto look = [&](int64_t s) {
-    if (s < 1 || s > 64 || (s > 1 && s > pages / 2)) return;
+    if (s < 1 || s > 64 || (s > 1 && s > pages / 2)) return;  // a share has two pages at least
     const double waves = (double)((base * s + slots - 1) / slots);
     const double rounds = (double)((pages + 2 * s - 1) / (2 * s));
     const double cost = waves * (rounds * step_us + cta_us) + (s > 1 ? 2.0 + join_us * s : 0.0);
@@ -923,7 +923,7 @@ Plan make_plan(int B, int T, int HQ, int HK, int max_rows, int max_pages, int wi
   const int sms = ffb::sm_count();
   if (p.kernel == TC) {
     const double join = (double)T * HQ * (D + 2) * 4 * 2 / 5e6;  // written and read at about 5 TB/s
-    p.splits = plan_splits((int64_t)B * HK * p.tiles, pages, sms, 2.5, 6.0, join);
+    p.splits = plan_splits((int64_t)B * HK * p.tiles, pages, sms, 2.0, 6.0, join);
     p.ctas = B * HK * p.splits;
     p.bytes = p.splits > 1 ? (int64_t)p.splits * T * HQ * (D + 2) * 4 : 0;
   } else {

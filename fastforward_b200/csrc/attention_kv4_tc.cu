@@ -70,6 +70,16 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// One thread of the (converged) warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
+}
 // fp32 pairs in one instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 r;
@@ -172,7 +182,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  constexpr uint32_t tmem = 0;  // all 512 columns are this CTA's, so they start at 0
   pdl_wait();
   if (tid == 0) pdl_launch();
 
@@ -206,7 +216,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
         int bad_pair = 0;
         for (int i = 0; i < 2 * nblk; ++i) {
           const uint32_t u = 2 * blk0 + i, s = u % RAW;
-          if (u >= RAW && !mbar_wait_bounded(&raw_empty[s], ((u / RAW) & 1u) ^ 1u, abort_flag)) {
+          if (u >= RAW && !wait_held(&raw_empty[s], ((u / RAW) & 1u) ^ 1u, abort_flag)) {
             *abort_flag = 1;
             break;
           }
@@ -239,66 +249,69 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
       }
     } else if (warp == 1) {
       // ---------------------------------------------------------------- MMAs
-      if (lane == 0) {
-        constexpr uint32_t idesc_s = idesc_bf16(128, 128);
-        constexpr uint32_t idesc_o = idesc_bf16(128, 128) | (1u << 16);  // B (= V) MN-major
-        auto wait_slot = [&](uint32_t u) {
-          if (!mbar_wait_bounded(&slot_full[u % SLOTS], (u / SLOTS) & 1u, abort_flag)) return false;
-          tc_fence_after();
-          return true;
-        };
-        auto issue_s = [&](int x, uint32_t u) {
-          const uint32_t qa = smem_u32(sq + x * TILE), kb = smem_u32(slots + (u % SLOTS) * TILE);
+      // The whole warp walks the blocks and one elected thread issues, so that descriptors and
+      // addresses stay in uniform registers: issued by one diverged thread an MMA took 130 clocks
+      // whatever its size.
+      constexpr uint32_t idesc_s = idesc_bf16(128, 128);
+      constexpr uint32_t idesc_o = idesc_bf16(128, 128) | (1u << 16);  // B (= V) MN-major
+      const uint32_t qbase = smem_u32(sq), kvbase = smem_u32(slots);
+      const bool leader = elect_one();
+      auto wait_uniform = [&](uint64_t* bar, uint32_t parity) {
+        const bool done = __all_sync(0xffffffffu, wait_held(bar, parity, abort_flag)) != 0;
+        tc_fence_after();
+        return done;
+      };
+      auto wait_slot = [&](uint32_t u) { return wait_uniform(&slot_full[u % SLOTS], (u / SLOTS) & 1u); };
+      auto scores = [&](int x, uint32_t u, bool free_slot) {
+        const uint64_t qd = umma_desc_sw128(qbase + x * TILE), kd = umma_desc_sw128(kvbase + (u % SLOTS) * TILE);
+        if (leader) {
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)
-            umma_f16(tmem + 128 * x, umma_desc_sw128(qa + (kk >> 2) * HALF + (kk & 3) * 32),
-                     umma_desc_sw128(kb + (kk >> 2) * HALF + (kk & 3) * 32), idesc_s, kk > 0 ? 1u : 0u);
+            umma_f16(128 * x, qd + ((kk >> 2) * HALF + (kk & 3) * 32) / 16, kd + ((kk >> 2) * HALF + (kk & 3) * 32) / 16, idesc_s,
+                     kk > 0 ? 1u : 0u);
           umma_commit(&s_full[x]);
-        };
-        auto issue_o = [&](int x, uint32_t u, bool first) {
-          const uint32_t vb = smem_u32(slots + (u % SLOTS) * TILE);
+          if (free_slot) umma_commit(&slot_empty[u % SLOTS]);
+        }
+        __syncwarp();
+      };
+      auto product = [&](int x, uint32_t u, bool first, bool free_slot) {
+        const uint64_t vd = umma_desc_sw128_mn(kvbase + (u % SLOTS) * TILE, HALF);
+        if (leader) {
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)
-            umma_f16_ts(tmem + 256 + 128 * x, tmem + 128 * x + 8 * kk, umma_desc_sw128_mn(vb + kk * 2048, HALF), idesc_o,
-                        (!first || kk > 0) ? 1u : 0u);
+            umma_f16_ts(256 + 128 * x, 128 * x + 8 * kk, vd + kk * 2048 / 16, idesc_o, (!first || kk > 0) ? 1u : 0u);
           umma_commit(&o_done[x]);
-        };
-        bool go = true;
-        if (nblk > 0) {
-          go = mbar_wait_bounded(&q_full[0], tiles & 1u, abort_flag) &&
-               (!two || mbar_wait_bounded(&q_full[1], tilesB & 1u, abort_flag)) && wait_slot(2 * blk0);
-          if (go) {
-            issue_s(0, 2 * blk0);
-            if (two) issue_s(1, 2 * blk0);
-            umma_commit(&slot_empty[(2 * blk0) % SLOTS]);
-          }
+          if (free_slot) umma_commit(&slot_empty[u % SLOTS]);
         }
-        for (int j = 0; j < nblk && go; ++j) {
-          const uint32_t uv = 2 * (blk0 + j) + 1, uk = uv + 1;
-          go = wait_slot(uv) && mbar_wait_bounded(&p_full[0], (blk0 + j) & 1u, abort_flag);
-          if (!go) break;
-          tc_fence_after();
-          issue_o(0, uv, j == 0);
-          const bool more = j + 1 < nblk;
-          if (more) {
-            go = wait_slot(uk);
-            if (!go) break;
-            issue_s(0, uk);
-          }
-          if (two) {
-            go = mbar_wait_bounded(&p_full[1], (blkB0 + j) & 1u, abort_flag);
-            if (!go) break;
-            tc_fence_after();
-            issue_o(1, uv, j == 0);
-          }
-          umma_commit(&slot_empty[uv % SLOTS]);
-          if (more) {
-            if (two) issue_s(1, uk);
-            umma_commit(&slot_empty[uk % SLOTS]);
-          }
+        __syncwarp();
+      };
+      bool go = true;
+      if (nblk > 0) {
+        go = wait_uniform(&q_full[0], tiles & 1u) && (!two || wait_uniform(&q_full[1], tilesB & 1u)) && wait_slot(2 * blk0);
+        if (go) {
+          scores(0, 2 * blk0, !two);
+          if (two) scores(1, 2 * blk0, true);
         }
-        if (!go) *abort_flag = 1;
       }
+      for (int j = 0; j < nblk && go; ++j) {
+        const uint32_t uv = 2 * (blk0 + j) + 1, uk = uv + 1;
+        const bool more = j + 1 < nblk;
+        go = wait_slot(uv) && wait_uniform(&p_full[0], (blk0 + j) & 1u);
+        if (!go) break;
+        product(0, uv, j == 0, !two);
+        if (more) {
+          go = wait_slot(uk);
+          if (!go) break;
+          scores(0, uk, !two);
+        }
+        if (two) {
+          go = wait_uniform(&p_full[1], (blkB0 + j) & 1u);
+          if (!go) break;
+          product(1, uv, j == 0, true);
+          if (more) scores(1, uk, true);
+        }
+      }
+      if (!go) *abort_flag = 1;
     } else if (warp >= 12) {
       // ---------------------------------------------------------------- dequantisation
       const int w = warp - 12;
@@ -306,13 +319,13 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
 #pragma unroll 1
         for (int is_v = 0; is_v < 2; ++is_v) {
           const uint32_t u = 2 * (blk0 + j) + is_v;
-          bool got = u < SLOTS || mbar_wait_bounded(&slot_empty[u % SLOTS], ((u / SLOTS) & 1u) ^ 1u, abort_flag);
+          bool got = u < SLOTS || wait_held(&slot_empty[u % SLOTS], ((u / SLOTS) & 1u) ^ 1u, abort_flag);
           got = __all_sync(0xffffffffu, got);  // one verdict for the warp
           uint8_t* dst = slots + (u % SLOTS) * TILE;
 #pragma unroll 1
           for (int a = 0; a < 2 && got; ++a) {
             const uint32_t ur = 2 * (blk0 + j) + a, s = ur % RAW;
-            got = mbar_wait_bounded(&raw_full[s], (ur / RAW) & 1u, abort_flag);
+            got = wait_held(&raw_full[s], (ur / RAW) & 1u, abort_flag);
             got = __all_sync(0xffffffffu, got);
             if (!got) break;
             const uint8_t* rec = raw + s * RECORD;
@@ -395,6 +408,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
         // no product would keep its warps from staging output over rows that others still write
         if (nblk > 0) {
           const uint32_t flip = args.scale_log2 < 0.f ? 0x80008000u : 0u;
+#pragma unroll
           for (int k = 0; k < 32; k += 2) {
             const int rr = quarter * 32 + k + (lane >> 4), cc = c0 + 128 * x + rr, ch = lane & 15;
             uint4 v = make_uint4(0u, 0u, 0u, 0u);
@@ -416,7 +430,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
         float m = -INFINITY, neg = 0.f, l = 0.f;  // neg: -m, 0 while nothing has been seen
         const float2 sc2 = make_float2(sc, sc);
         for (int j = 0; j < nblk; ++j) {
-          if (!__all_sync(0xffffffffu, mbar_wait_bounded(&s_full[x], (base_blk + j) & 1u, abort_flag) && !*abort_flag)) {
+          if (!__all_sync(0xffffffffu, wait_held(&s_full[x], (base_blk + j) & 1u, abort_flag) && !*abort_flag)) {
             ok = false;
             break;
           }
@@ -461,7 +475,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
             m = nm;
             neg = m == -INFINITY ? 0.f : -m;
             if (j > 0) {
-              if (!__all_sync(0xffffffffu, mbar_wait_bounded(&o_done[x], (base_blk + j - 1) & 1u, abort_flag))) {
+              if (!__all_sync(0xffffffffu, wait_held(&o_done[x], (base_blk + j - 1) & 1u, abort_flag))) {
                 ok = false;
                 break;
               }
@@ -510,7 +524,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
           if (lane == 0) mbar_arrive(&p_full[x]);
         }
         if (ok && nblk > 0)
-          ok = __all_sync(0xffffffffu, mbar_wait_bounded(&o_done[x], (base_blk + nblk - 1) & 1u, abort_flag) && !*abort_flag);
+          ok = __all_sync(0xffffffffu, wait_held(&o_done[x], (base_blk + nblk - 1) & 1u, abort_flag) && !*abort_flag);
         if (!ok) *abort_flag = 1;
         if (ok) {
           tc_fence_after();
@@ -584,11 +598,15 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
     }
   }
 
-  if (warp == 1 && lane == 0) {
-    // every MMA issued has completed before tensor and shared memory are released
-    volatile int never = 0;
-    umma_commit(last);
-    mbar_wait_bounded(last, 0, &never, 200000000ull);
+  if (warp == 1) {
+    // every MMA issued has completed before tensor and shared memory are released (the thread that
+    // elect_one names is the same every time)
+    if (elect_one()) {
+      volatile int never = 0;
+      umma_commit(last);
+      mbar_wait_bounded(last, 0, &never, 200000000ull);
+    }
+    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();

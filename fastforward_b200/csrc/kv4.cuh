@@ -95,6 +95,25 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                "l"(src), "r"(bytes), "r"(smem_u32(bar))
                : "memory");
 }
+// mbar_wait_bounded for waits that are expected to take long: the hardware may hold the thread for up
+// to 10 us a try, so that waiting warps leave the issue slots to the others.
+__device__ __forceinline__ bool wait_held(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = global_timer_ns();
+  for (uint32_t i = 0; i < (1u << 24); ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(10000u)
+        : "memory");
+    if (ok) return true;
+    if (*abort || global_timer_ns() - t0 > 2000000000ull) return false;
+  }
+  return false;
+}
 // The pages that a tile of rows [first, last] (positions) reads: the first n_sink pages, then
 // [first_page, first_page + n - n_sink).
 struct PageSet {
