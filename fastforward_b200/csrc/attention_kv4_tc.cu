@@ -68,6 +68,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // One thread of the (converged) warp.
@@ -314,83 +319,82 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
       if (!go) *abort_flag = 1;
     } else if (warp >= 12) {
       // ---------------------------------------------------------------- dequantisation
-      const int w = warp - 12;
+      const int r8 = 8 * (warp - 12);  // this warp's eight tokens of a page
+      // K: token pairs (r, r ^ 5) x four chunks meet all banks on the load and on the store;
+      // V: tokens {0, 1, 6, 7} / {2, 3, 4, 5} of eight x two neighbouring 16-byte pairs
+      const int kt = lane & 3, kr = r8 + ((lane >> 3) ^ ((lane & 4) ? 5 : 0));
+      const int vk = (lane >> 1) & 3, pair = 2 * (lane >> 4) + (lane & 1);
+      const int vr = r8 + ((lane & 8) ? 2 + vk : (vk < 2 ? vk : 4 + vk));
       for (int j = 0; j < nblk && ok; ++j) {
-#pragma unroll 1
+        const uint32_t u = 2 * (blk0 + j);  // the K tile's number, and the first page's
+        // tokens past the newest row's position are held by nobody: whatever is there is not used
+        int live[2];
+        bool got = true;
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+          got = got && wait_held(&raw_full[(u + a) % RAW], ((u + a) / RAW) & 1u, abort_flag);
+          const int key0 = i0 + 2 * j + a < i1 ? page_index(i0 + 2 * j + a) * PAGE : 0;
+          live[a] = raw_bad[(u + a) % RAW] ? 0 : min(max(ps.kend - key0, 0), PAGE);
+        }
+#pragma unroll
         for (int is_v = 0; is_v < 2; ++is_v) {
-          const uint32_t u = 2 * (blk0 + j) + is_v;
-          bool got = u < SLOTS || wait_held(&slot_empty[u % SLOTS], ((u / SLOTS) & 1u) ^ 1u, abort_flag);
+          const uint32_t slot = (u + is_v) % SLOTS;
+          got = got && (u + is_v < SLOTS || wait_held(&slot_empty[slot], (((u + is_v) / SLOTS) & 1u) ^ 1u, abort_flag));
           got = __all_sync(0xffffffffu, got);  // one verdict for the warp
-          uint8_t* dst = slots + (u % SLOTS) * TILE;
-#pragma unroll 1
-          for (int a = 0; a < 2 && got; ++a) {
-            const uint32_t ur = 2 * (blk0 + j) + a, s = ur % RAW;
-            got = wait_held(&raw_full[s], (ur / RAW) & 1u, abort_flag);
-            got = __all_sync(0xffffffffu, got);
-            if (!got) break;
-            const uint8_t* rec = raw + s * RECORD;
-            const bool bad = raw_bad[s];
-            const int key0 = i0 + 2 * j + a < i1 ? page_index(i0 + 2 * j + a) * PAGE : 0;
-            // tokens past the newest row's position are held by nobody: whatever is there is not used
-            const int live = bad ? 0 : min(max(ps.kend - key0, 0), PAGE);
-            {
-              const int r8 = 8 * w;  // this warp's eight tokens
-              if (!is_v) {
-                // token pairs (r, r ^ 5) x four chunks meet all banks on the load and on the store
-                const int k = lane >> 3, e = (lane >> 2) & 1, t = lane & 3;
-                const int r = r8 + (k ^ (e ? 5 : 0)) , row = 64 * a + r;
-                uint4 c = make_uint4(0u, 0u, 0u, 0u);
-                uint2 sc = make_uint2(0u, 0u);
-                if (r < live) {
-                  c = *reinterpret_cast<const uint4*>(rec + 64 * r + 16 * t);
-                  sc = *reinterpret_cast<const uint2*>(rec + K_SCALES + 8 * r);
-                  const uint2 vs = *reinterpret_cast<const uint2*>(rec + V_SCALES + 8 * r);
-                  if (not_finite2(vs.x) || not_finite2(vs.y)) sc = make_uint2(0x7fc07fc0u, 0x7fc07fc0u);
-                }
-                const uint32_t words[4] = {c.x, c.y, c.z, c.w};
-                const uint32_t scale[4] = {__byte_perm(sc.x, 0, 0x1010), __byte_perm(sc.x, 0, 0x3232),
-                                           __byte_perm(sc.y, 0, 0x1010), __byte_perm(sc.y, 0, 0x3232)};
+          if (!got) break;
+          uint8_t* dst = slots + slot * TILE;
+          // both pages' loads first: one after the other their latencies bound the whole kernel
+          uint4 c[2];
+          uint2 sc[2];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                  const int chunk = 4 * (q & 1) + t;
-                  *reinterpret_cast<uint4*>(dst + (q >> 1) * HALF + row * 128 + ((chunk ^ (row & 7)) << 4)) =
-                      dequant8(words[q], scale[q]);
-                }
-              } else {
-                // tokens {0, 1, 6, 7} / {2, 3, 4, 5} of eight x two neighbouring 16-byte pairs
-                const int k = (lane >> 1) & 3, set = (lane >> 3) & 1, pair = 2 * (lane >> 4) + (lane & 1);
-                const int r = r8 + (set ? 2 + k : (k < 2 ? k : 4 + k)), row = 64 * a + r;
-                uint4 c = make_uint4(0u, 0u, 0u, 0u);
-                uint2 sc = make_uint2(0u, 0u);
-                if (r < live) {
-                  c = *reinterpret_cast<const uint4*>(rec + V_CODES + 64 * r + 16 * (pair ^ ((r & 4) >> 1)));
-                  sc = *reinterpret_cast<const uint2*>(rec + V_SCALES + 8 * r);
-                  if (not_finite2(sc.x) || not_finite2(sc.y)) sc = make_uint2(0u, 0u);
-                }
-                const uint32_t words[4] = {c.x, c.y, c.z, c.w};  // chunks 2 pair, 2 pair + 1, two words each
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                  const int chunk = 4 * (pair & 1) + q;
-                  *reinterpret_cast<uint4*>(dst + (pair >> 1) * HALF + row * 128 + ((chunk ^ (row & 7)) << 4)) =
-                      dequant8(words[q], (q & 1) ? sc.y : sc.x);
-                }
-              }
+          for (int a = 0; a < 2; ++a) {
+            const uint8_t* rec = raw + ((u + a) % RAW) * RECORD;
+            c[a] = make_uint4(0u, 0u, 0u, 0u);
+            sc[a] = make_uint2(0u, 0u);
+            if (!is_v && kr < live[a]) {
+              c[a] = *reinterpret_cast<const uint4*>(rec + 64 * kr + 16 * kt);
+              sc[a] = *reinterpret_cast<const uint2*>(rec + K_SCALES + 8 * kr);
+              const uint2 vs = *reinterpret_cast<const uint2*>(rec + V_SCALES + 8 * kr);
+              if (not_finite2(vs.x) || not_finite2(vs.y)) sc[a] = make_uint2(0x7fc07fc0u, 0x7fc07fc0u);
+            }
+            if (is_v && vr < live[a]) {
+              c[a] = *reinterpret_cast<const uint4*>(rec + V_CODES + 64 * vr + 16 * (pair ^ ((vr & 4) >> 1)));
+              sc[a] = *reinterpret_cast<const uint2*>(rec + V_SCALES + 8 * vr);
+              if (not_finite2(sc[a].x) || not_finite2(sc[a].y)) sc[a] = make_uint2(0u, 0u);
             }
           }
-          if (!got) {
-            ok = false;
-            *abort_flag = 1;
-            break;
+#pragma unroll
+          for (int a = 0; a < 2; ++a) {
+            const uint32_t words[4] = {c[a].x, c[a].y, c[a].z, c[a].w};
+            if (!is_v) {
+              const uint32_t scale[4] = {__byte_perm(sc[a].x, 0, 0x1010), __byte_perm(sc[a].x, 0, 0x3232),
+                                         __byte_perm(sc[a].y, 0, 0x1010), __byte_perm(sc[a].y, 0, 0x3232)};
+              uint8_t* row = dst + (64 * a + kr) * 128;
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<uint4*>(row + (q >> 1) * HALF + (((4 * (q & 1) + kt) ^ (kr & 7)) << 4)) =
+                    dequant8(words[q], scale[q]);
+            } else {  // chunks 2 pair, 2 pair + 1 of V, two words each
+              uint8_t* row = dst + (pair >> 1) * HALF + (64 * a + vr) * 128;
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<uint4*>(row + (((4 * (pair & 1) + q) ^ (vr & 7)) << 4)) =
+                    dequant8(words[q], (q & 1) ? sc[a].y : sc[a].x);
+            }
           }
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
-            mbar_arrive(&slot_full[u % SLOTS]);
+            mbar_arrive(&slot_full[slot]);
             if (is_v) {
-              mbar_arrive(&raw_empty[(2 * (blk0 + j)) % RAW]);
-              mbar_arrive(&raw_empty[(2 * (blk0 + j) + 1) % RAW]);
+              mbar_arrive(&raw_empty[u % RAW]);
+              mbar_arrive(&raw_empty[(u + 1) % RAW]);
             }
           }
+        }
+        if (!got) {
+          ok = false;
+          *abort_flag = 1;
         }
       }
     } else if (warp >= 4) {
@@ -444,29 +448,38 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
           const bool whole = bad == 0 && seen_by_all(ka) && seen_by_all(kb);
           // columns of this row that count, per page: c <= hi and (c >= lo or c < sk)
           const int top = min(pos, ps.kend - 1), low = args.window > 0 ? pos - args.window + 1 : 0;
-          const int hi[2] = {(bad & 1) ? -1 : top - ka, (bad & 2) ? -1 : top - kb};
-          const int lo[2] = {low - ka, low - kb}, sk[2] = {args.sinks - ka, args.sinks - kb};
+          if (!whole) {  // rare blocks: the scores that do not count become -inf where they lie
+            const int hi[2] = {(bad & 1) ? -1 : top - ka, (bad & 2) ? -1 : top - kb};
+            const int lo[2] = {low - ka, low - kb}, sk[2] = {args.sinks - ka, args.sinks - kb};
+#pragma unroll 1
+            for (int q = 0; q < 8; ++q) {
+              const int first = 16 * (q & 3), h = hi[q >> 2] - first, l0 = lo[q >> 2] - first, s0 = sk[q >> 2] - first;
+              uint32_t y[16];
+              tmem_ld16_async(st + 16 * q, y);
+              tmem_wait_ld();
+              reg_fence(y);
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                if (!(e <= h && (e >= l0 || e < s0))) y[e] = 0xff800000u;
+              tmem_st16(st + 16 * q, y);
+            }
+            tmem_wait_st();
+          }
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          uint32_t v[2][32];
+          tmem_ld32_async(st, v[0]);
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            uint32_t v[32];
-            tmem_ld32_async(st + 32 * q, v);
             tmem_wait_ld();
-            reg_fence(v);
-            if (whole) {
+            reg_fence(v[q & 1]);
+            if (q < 3) tmem_ld32_async(st + 32 * (q + 1), v[(q + 1) & 1]);
 #pragma unroll
-              for (int e = 0; e < 32; e += 2)
-                mx[(e >> 1) & 3] = fmaxf(mx[(e >> 1) & 3], fmaxf(__uint_as_float(v[e]), __uint_as_float(v[e + 1])));
-            } else {
-#pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                const int c = 32 * (q & 1) + e;
-                if (c <= hi[q >> 1] && (c >= lo[q >> 1] || c < sk[q >> 1])) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(v[e]));
-              }
-            }
+            for (int e = 0; e < 32; e += 2)
+              mx[(e >> 1) & 3] = fmaxf(mx[(e >> 1) & 3], fmaxf(__uint_as_float(v[q & 1][e]), __uint_as_float(v[q & 1][e + 1])));
           }
-          float bmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-          bmax = bmax == -INFINITY ? bmax : bmax * sc;
+          uint32_t w[2][16];  // the scores again, for the probabilities: on their way while the maximum is looked at
+          tmem_ld16_async(st, w[0]);
+          const float bmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
           const bool grow = bmax > m + LAZY;
           if (__any_sync(0xffffffffu, grow)) {
             const float nm = grow ? bmax : m;
@@ -482,13 +495,13 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
               tc_fence_after();
 #pragma unroll 1
               for (int q = 0; q < 8; ++q) {
-                uint32_t w[16];
-                tmem_ld16_async(ot + 16 * q, w);
+                uint32_t y[16];
+                tmem_ld16_async(ot + 16 * q, y);
                 tmem_wait_ld();
-                reg_fence(w);
+                reg_fence(y);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(__uint_as_float(w[e]) * alpha);
-                tmem_st16(ot + 16 * q, w);
+                for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(__uint_as_float(y[e]) * alpha);
+                tmem_st16(ot + 16 * q, y);
               }
               tmem_wait_st();
             }
@@ -496,26 +509,19 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
           const float2 neg2 = make_float2(neg, neg);
           float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t v[32], p[16];
-            tmem_ld32_async(st + 32 * q, v);
+          for (int q = 0; q < 8; ++q) {
+            uint32_t p[8];
             tmem_wait_ld();
-            reg_fence(v);
-            if (!whole) {
+            reg_fence(w[q & 1]);
+            if (q < 7) tmem_ld16_async(st + 16 * (q + 1), w[(q + 1) & 1]);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) {
-                const int c = 32 * (q & 1) + e;
-                if (!(c <= hi[q >> 1] && (c >= lo[q >> 1] || c < sk[q >> 1]))) v[e] = 0xff800000u;  // -inf
-              }
-            }
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              const float2 y = fma2(make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), sc2, neg2);
+            for (int e = 0; e < 16; e += 2) {
+              const float2 y = fma2(make_float2(__uint_as_float(w[q & 1][e]), __uint_as_float(w[q & 1][e + 1])), sc2, neg2);
               const float2 z = make_float2(ex2(y.x), ex2(y.y));
               sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], z);
               p[e >> 1] = pack_bf16(z.x, z.y);
             }
-            tmem_st16(st + 16 * q, p);
+            tmem_st8(st + 8 * q, p);
           }
           l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
           tmem_wait_st();
