@@ -4,11 +4,18 @@
 //   n = x / sqrt(mean(x^2) + eps) * w,  y[i] = n[i] c[i] - n[i + 64] s[i]   (i < 64)
 //                                       y[i] = n[i] c[i] + n[i - 64] s[i]   (i >= 64)
 // with the queries rounded once to bf16 and the keys and values quantised straight into the
-// cache.  Sixteen lanes take one (row, head): lane i holds channels 4i..4i+3 and 64+4i..,
-// so the rotation needs no exchange and a scale group is eight lanes.  Keys are computed in
-// fp64 up to their codes: a key next to the border of two codes gets the same code whatever
-// the order of operations (fp64 arithmetic is an eighth of the pass's heads' work).
-// Bound by HBM: a row reads 256 (HQ + 2 HK) + 512 bytes and writes 256 HQ + 144 HK.
+// cache.  Bound by HBM: a row reads 256 (HQ + 2 HK) + 512 bytes and writes 256 HQ + 144 HK.
+// Sixteen lanes take one (row, head): lane i holds channels 4i..4i+3 and 64+4i.., so the
+// rotation needs no exchange and a scale group is eight lanes.  A CTA takes one row: the first
+// ones of a row its query heads (four to a half warp once there are enough rows, their loads
+// issued together), the last its key and value heads.
+//
+// The codes are those of the formula in exact arithmetic, up to fp64's rounding: a key next to
+// the border of two codes must not fall to either side by chance.  x w is exact in fp32 (two
+// bf16), so is its product with the bf16 cosine (24 bits); only the difference of the two
+// products and the norm's factor are fp64.  Everything after that is fp32, with the distance to
+// the next border looked at, and done again in fp64 where that distance is within fp32's error
+// (about one head in a thousand).  Values are bf16: x - q s is exact, so borders are seen as such.
 #include "kv4.cuh"
 #include "pdl.cuh"
 
@@ -33,40 +40,80 @@ __device__ __forceinline__ float up5(float v) {
   const uint32_t b = __float_as_uint(v), low = (1u << 19) - 1;
   return __uint_as_float((b + low) & ~low);
 }
-__device__ __forceinline__ double quotient(double x, double s) { return x / s; }
-__device__ __forceinline__ float quotient(float x, float s) { return __fdiv_rn(x, s); }
+// (int) code of x under the scale s = 1 / r from t = x r: the nearest integer, and whether t lies too
+// near the border of two for fp32 to tell.
+__device__ __forceinline__ int code_of(float t, bool& close) {
+  const float q = rintf(t);
+  close |= fabsf(fabsf(t - q) - 0.5f) < 4e-6f;  // |t| <= 7: y r is within 3 x 2^-24 x 7 of the quotient
+  return (int)fminf(fmaxf(q, -7.f), 7.f);
+}
+__device__ __forceinline__ float group_max(float top, uint32_t mask) {
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(mask, top, o));
+  return top;
+}
+constexpr float BIG = 1.7014118346046923e38f;    // 2^127
+constexpr float SMALL = 7.888609052210118e-31f;  // 2^-100
 
 // Scale and nibbles (lowest first) of this lane's four values of a group held by eight lanes.
-template <typename F>
-__device__ __forceinline__ uint32_t group_codes(const F (&y)[4], uint32_t mask, float& scale) {
-  const F big = (F)1.7014118346046923e38;  // 2^127
-  F top = 0;
+// Values: bf16, exact.
+__device__ __forceinline__ uint32_t value_codes(const float (&y)[4], uint32_t mask, float& scale) {
+  float top = 0.f;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const F a = y[e] < 0 ? -y[e] : y[e];
-    top = a < big ? (a > top ? a : top) : (F)INFINITY;  // a NaN fails the comparison too
-  }
-#pragma unroll
-  for (int o = 1; o < 8; o <<= 1) {
-    const F other = __shfl_xor_sync(mask, top, o);
-    top = other > top ? other : top;
-  }
-  if (!(top < big)) {
-    scale = __uint_as_float(0x7fc00000u);
+  for (int e = 0; e < 4; ++e) top = fabsf(y[e]) < BIG ? fmaxf(top, fabsf(y[e])) : INFINITY;  // a NaN fails it too
+  top = group_max(top, mask);
+  if (!(top < BIG) || top < SMALL) {
+    scale = top < BIG ? 0.f : __uint_as_float(0x7fc00000u);
     return 0x8888u;
   }
-  if (top < (F)7.888609052210118e-31) {  // 2^-100
-    scale = 0.f;
-    return 0x8888u;
-  }
-  const F s = up5(quotient(top, (F)7));
-  scale = (float)s;
+  // (a bf16 over 7 is never so near a number of five bits that fp32's quotient crosses it)
+  const float s = up5(__fdiv_rn(top, 7.f)), r = __frcp_rn(s), half = 0.5f * s;
+  scale = s;
   uint32_t codes = 0;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const int q = (int)rint(quotient(y[e], s));
-    codes |= (uint32_t)(min(max(q, -7), 7) + 8) << (4 * e);
+    // q from the approximate quotient is one off at most; the rest x - q s is exact and tells
+    float q = rintf(y[e] * r);
+    const float rest = fmaf(-q, s, y[e]), off = fabsf(rest);
+    if (off > half || (off == half && ((int)q & 1))) q += rest > 0.f ? 1.f : -1.f;
+    codes |= (uint32_t)((int)fminf(fmaxf(q, -7.f), 7.f) + 8) << (4 * e);
   }
+  return codes;
+}
+// Keys: fp64.
+__device__ __forceinline__ uint32_t key_codes(const double (&y)[4], uint32_t mask, float& scale) {
+  float f[4], top = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    f[e] = (float)y[e];
+    top = fabsf(f[e]) < BIG ? fmaxf(top, fabsf(f[e])) : INFINITY;
+  }
+  top = group_max(top, mask);
+  if (!(top < BIG) || top < SMALL) {
+    scale = top < BIG ? 0.f : __uint_as_float(0x7fc00000u);
+    return 0x8888u;
+  }
+  const float seventh = __fdiv_rn(top, 7.f);
+  float s = up5(seventh);
+  const uint32_t low = (__float_as_uint(seventh) + 8u) & ((1u << 19) - 1);
+  bool close = low < 16u;  // within 8 units of a number of five bits
+  const float r = __frcp_rn(s);
+  uint32_t codes = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) codes |= (uint32_t)(code_of(f[e] * r, close) + 8) << (4 * e);
+  if (__any_sync(mask, close)) {  // in fp64
+    double most = 0.0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) most = fmax(most, fabs(y[e]));
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) most = fmax(most, __shfl_xor_sync(mask, most, o));
+    const double exact = up5(most / 7.0);
+    s = (float)exact;
+    codes = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) codes |= (uint32_t)((int)fmin(fmax(rint(y[e] / exact), -7.0), 7.0) + 8) << (4 * e);
+  }
+  scale = s;
   return codes;
 }
 
@@ -118,78 +165,122 @@ struct WriteArgs {
   Seqs seqs;
 };
 
+// Sum over the sixteen lanes of one (row, head).
 template <typename F>
-__device__ __forceinline__ void norm_rotate(const float (&xa)[4], const float (&xb)[4], const uint16_t* w,
-                                            const uint16_t* cr, const uint16_t* sr, float eps, int i, uint32_t mask,
-                                            F (&ya)[4], F (&yb)[4]) {
-  double ss = 0.0;  // bf16 squares are exact in fp32, their fp64 sum does not depend on its order
+__device__ __forceinline__ F head_sum(F v, uint32_t mask) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) ss += (double)(xa[e] * xa[e]) + (double)(xb[e] * xb[e]);
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) ss += __shfl_xor_sync(mask, ss, o);
-  const F inv = (F)(1.0 / sqrt(ss / D + (double)eps));
-  float wa[4], wb[4], ca[4], cb[4], sa[4], sb[4];
-  unpack4(__ldg(reinterpret_cast<const uint2*>(w + 4 * i)), wa);
-  unpack4(__ldg(reinterpret_cast<const uint2*>(w + 64 + 4 * i)), wb);
-  unpack4(__ldg(reinterpret_cast<const uint2*>(cr + 4 * i)), ca);
-  unpack4(__ldg(reinterpret_cast<const uint2*>(cr + 64 + 4 * i)), cb);
-  unpack4(__ldg(reinterpret_cast<const uint2*>(sr + 4 * i)), sa);
-  unpack4(__ldg(reinterpret_cast<const uint2*>(sr + 64 + 4 * i)), sb);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const F na = (F)xa[e] * inv * (F)wa[e], nb = (F)xb[e] * inv * (F)wb[e];
-    ya[e] = na * (F)ca[e] - nb * (F)sa[e];
-    yb[e] = nb * (F)cb[e] + na * (F)sb[e];
-  }
+  for (int o = 1; o < 16; o <<= 1) v += __shfl_xor_sync(mask, v, o);
+  return v;
 }
 
-__global__ void __launch_bounds__(WARPS * 32) kv4_write_kernel(const WriteArgs p) {
+struct Turn {  // this lane's cosines and sines of a row
+  float ca[4], cb[4], sa[4], sb[4];
+};
+__device__ __forceinline__ void load_turn(const WriteArgs& p, int t, int i, Turn& r) {
+  const int64_t at = (int64_t)t * D + 4 * i;
+  unpack4(__ldg(reinterpret_cast<const uint2*>(p.cos + at)), r.ca);
+  unpack4(__ldg(reinterpret_cast<const uint2*>(p.cos + at + 64)), r.cb);
+  unpack4(__ldg(reinterpret_cast<const uint2*>(p.sin + at)), r.sa);
+  unpack4(__ldg(reinterpret_cast<const uint2*>(p.sin + at + 64)), r.sb);
+}
+
+// U: query heads of a half warp.
+template <int U>
+__global__ void __launch_bounds__(WARPS * 32, 4) kv4_write_kernel(const WriteArgs p, int q_chunks) {
   pdl_wait();
   pdl_launch();
-  const int lane = threadIdx.x & 31, i = lane & 15;
+  const int lane = threadIdx.x & 31, i = lane & 15, slot = threadIdx.x >> 4, t = blockIdx.x;
   const uint32_t mask = 0xffffu << (lane & 16);
-  const int heads = p.HQ + 2 * p.seqs.HK;
-  const int64_t item = ((int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5)) * 2 + (lane >> 4);
-  if (item >= (int64_t)p.seqs.T * heads) return;
-  const int t = (int)(item / heads), h = (int)(item - (int64_t)t * heads);
-  const int b = seq_of(p.seqs, t);
-  if (b < 0) return;
-  float xa[4], xb[4];
-  const uint16_t* x = p.qkv + t * p.row_stride + (int64_t)h * D;
-  unpack4(*reinterpret_cast<const uint2*>(x + 4 * i), xa);
-  unpack4(*reinterpret_cast<const uint2*>(x + 64 + 4 * i), xb);
-  const uint16_t* cr = p.cos + (int64_t)t * D;
-  const uint16_t* sr = p.sin + (int64_t)t * D;
-  if (h < p.HQ) {
-    float ya[4], yb[4];
-    norm_rotate(xa, xb, p.q_norm, cr, sr, p.eps, i, mask, ya, yb);
-    uint16_t* dst = p.yq + ((int64_t)h * p.seqs.T + t) * D;
-    *reinterpret_cast<uint2*>(dst + 4 * i) =
-        make_uint2((uint32_t)f2bf(ya[0]) | ((uint32_t)f2bf(ya[1]) << 16), (uint32_t)f2bf(ya[2]) | ((uint32_t)f2bf(ya[3]) << 16));
-    *reinterpret_cast<uint2*>(dst + 64 + 4 * i) =
-        make_uint2((uint32_t)f2bf(yb[0]) | ((uint32_t)f2bf(yb[1]) << 16), (uint32_t)f2bf(yb[2]) | ((uint32_t)f2bf(yb[3]) << 16));
+  const int HK = p.seqs.HK;
+  const uint16_t* x = p.qkv + t * p.row_stride + 4 * i;
+  if ((int)blockIdx.y < q_chunks) {
+    const int h0 = (blockIdx.y * 2 * WARPS + slot) * U;
+    uint2 ua[U], ub[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      ua[u] = ub[u] = make_uint2(0u, 0u);
+      if (h0 + u < p.HQ) {
+        ua[u] = __ldg(reinterpret_cast<const uint2*>(x + (int64_t)(h0 + u) * D));
+        ub[u] = __ldg(reinterpret_cast<const uint2*>(x + (int64_t)(h0 + u) * D + 64));
+      }
+    }
+    Turn r;
+    load_turn(p, t, i, r);
+    float wa[4], wb[4];
+    unpack4(__ldg(reinterpret_cast<const uint2*>(p.q_norm + 4 * i)), wa);
+    unpack4(__ldg(reinterpret_cast<const uint2*>(p.q_norm + 64 + 4 * i)), wb);
+    if (t < __ldg(p.seqs.row_start) || t >= __ldg(p.seqs.row_start + p.seqs.B)) return;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (h0 + u >= p.HQ) break;
+      float xa[4], xb[4], ss = 0.f;
+      unpack4(ua[u], xa);
+      unpack4(ub[u], xb);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) ss = fmaf(xa[e], xa[e], fmaf(xb[e], xb[e], ss));
+      const float inv = __frsqrt_rn(head_sum(ss, mask) * (1.f / D) + p.eps);
+      float ya[4], yb[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float na = xa[e] * inv * wa[e], nb = xb[e] * inv * wb[e];
+        ya[e] = na * r.ca[e] - nb * r.sa[e];
+        yb[e] = nb * r.cb[e] + na * r.sb[e];
+      }
+      uint16_t* dst = p.yq + ((int64_t)(h0 + u) * p.seqs.T + t) * D + 4 * i;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(ya[0], ya[1]), pack_bf16(ya[2], ya[3]));
+      *reinterpret_cast<uint2*>(dst + 64) = make_uint2(pack_bf16(yb[0], yb[1]), pack_bf16(yb[2], yb[3]));
+    }
     return;
   }
-  const bool is_v = h >= p.HQ + p.seqs.HK;
-  const int kvh = h - p.HQ - (is_v ? p.seqs.HK : 0);
+  const int pair = (blockIdx.y - q_chunks) * 2 * WARPS + slot;
+  if (pair >= 2 * HK) return;
+  const bool is_v = pair >= HK;
+  const int h = is_v ? pair - HK : pair;
+  const uint2 ua = __ldg(reinterpret_cast<const uint2*>(x + (int64_t)(p.HQ + pair) * D));
+  const uint2 ub = __ldg(reinterpret_cast<const uint2*>(x + (int64_t)(p.HQ + pair) * D + 64));
+  const int b = seq_of(p.seqs, t);
+  if (b < 0) return;
   const int64_t pos = (int64_t)__ldg(p.seqs.ctx_len + b) - (__ldg(p.seqs.row_start + b + 1) - t);
-  uint8_t* rec = record_of(p.seqs, b, pos, kvh);
+  uint8_t* rec = record_of(p.seqs, b, pos, h);
   if (!rec) {
     if (i == 0) atomicOr(&ffb_device_error_word, (uint32_t)ffb::ERR_KV4_PAGE);
     return;
   }
-  const int token = (int)(pos % PAGE);
-  float s_lo, s_hi;
-  uint32_t lo, hi;
+  const int token = (int)(pos & (PAGE - 1));
+  float xa[4], xb[4], s_lo, s_hi;
+  unpack4(ua, xa);
+  unpack4(ub, xb);
   if (is_v) {
-    lo = group_codes(xa, mask, s_lo);
-    hi = group_codes(xb, mask, s_hi);
+    const uint32_t lo = value_codes(xa, mask, s_lo), hi = value_codes(xb, mask, s_hi);
     store_v(rec + V_CODES + 64 * token, lo, hi, i, token, mask);
   } else {
+    Turn r;
+    load_turn(p, t, i, r);
+    float wa[4], wb[4];
+    unpack4(__ldg(reinterpret_cast<const uint2*>(p.k_norm + 4 * i)), wa);
+    unpack4(__ldg(reinterpret_cast<const uint2*>(p.k_norm + 64 + 4 * i)), wb);
+    double ss = 0.0;  // bf16 squares are exact in fp32, their fp64 sum does not depend on its order
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ss += (double)(xa[e] * xa[e]) + (double)(xb[e] * xb[e]);
+    ss = head_sum(ss, mask);
+    const double inv = 1.0 / sqrt(ss / D + (double)p.eps);
     double ya[4], yb[4];
-    norm_rotate(xa, xb, p.k_norm, cr, sr, p.eps, i, mask, ya, yb);
-    lo = group_codes(ya, mask, s_lo);
-    hi = group_codes(yb, mask, s_hi);
+    if (ss > 1e-20 && ss < 1e30) {  // no product below leaves fp32's range
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float ta = xa[e] * wa[e], tb = xb[e] * wb[e];
+        ya[e] = ((double)(ta * r.ca[e]) - (double)(tb * r.sa[e])) * inv;
+        yb[e] = ((double)(tb * r.cb[e]) + (double)(ta * r.sb[e])) * inv;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const double na = (double)xa[e] * inv * (double)wa[e], nb = (double)xb[e] * inv * (double)wb[e];
+        ya[e] = na * (double)r.ca[e] - nb * (double)r.sa[e];
+        yb[e] = nb * (double)r.cb[e] + na * (double)r.sb[e];
+      }
+    }
+    const uint32_t lo = key_codes(ya, mask, s_lo), hi = key_codes(yb, mask, s_hi);
     store_k(rec + 64 * token, lo, hi, i, mask);
   }
   if ((i & 7) == 0) {  // groups i / 8 (low channels) and 2 + i / 8
@@ -206,9 +297,8 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_read_kernel(const Seqs p, uint
   pdl_launch();
   const int lane = threadIdx.x & 31, i = lane & 15;
   const uint32_t mask = 0xffffu << (lane & 16);
-  const int64_t item = ((int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5)) * 2 + (lane >> 4);
-  if (item >= (int64_t)p.T * p.HK) return;
-  const int h = (int)(item / p.T), t = (int)(item - (int64_t)h * p.T);
+  const int t = (int)blockIdx.x * 2 * WARPS + (threadIdx.x >> 4), h = blockIdx.y;
+  if (t >= p.T) return;
   const int b = seq_of(p, t);
   if (b < 0) return;
   const int64_t pos = (int64_t)__ldg(p.ctx_len + b) - (__ldg(p.row_start + b + 1) - t);
@@ -285,9 +375,13 @@ extern "C" int ffb_qk_norm_rope_kv4(const uint16_t* qkv, int64_t row_stride, con
               "%s: qkv, norms, tables and yq must be 8-byte aligned", who);
   WriteArgs a = {qkv, row_stride, q_norm, k_norm, cos, sin, yq, eps, HQ,
                  {pages, page_table, row_start, ctx_len, num_pages, max_pages, B, T, HK, table_stride}};
-  const int64_t items = (int64_t)T * (HQ + 2 * HK), grid = (items + 2 * WARPS - 1) / (2 * WARPS);
-  FFB_REQUIRE(grid <= 0x7fffffff, "%s: T=%d HQ=%d HK=%d too large", who, T, HQ, HK);
-  cudaError_t e = ffb::launch(kv4_write_kernel, dim3((unsigned)grid), dim3(WARPS * 32), 0, (cudaStream_t)stream, a);
+  // with few rows every half warp has one head: 320 rows take 10 us so, and 7000 rows a third less
+  // with four
+  const bool many = T >= 4 * ffb::sm_count();
+  const int heads = (many ? 4 : 1) * 2 * WARPS, q_chunks = (HQ + heads - 1) / heads;
+  const dim3 grid(T, q_chunks + (2 * HK + 2 * WARPS - 1) / (2 * WARPS));
+  cudaError_t e = many ? ffb::launch(kv4_write_kernel<4>, grid, dim3(WARPS * 32), 0, (cudaStream_t)stream, a, q_chunks)
+                       : ffb::launch(kv4_write_kernel<1>, grid, dim3(WARPS * 32), 0, (cudaStream_t)stream, a, q_chunks);
   if (e != cudaSuccess) return ffb::fail(FFB_ECUDA, "%s: %s", who, cudaGetErrorString(e));
   return FFB_OK;
 }
@@ -301,9 +395,8 @@ extern "C" int ffb_kv4_read(const uint8_t* pages, int num_pages, const int* page
   FFB_REQUIRE(k && v, "%s: NULL pointer", who);
   FFB_REQUIRE(ffb::aligned(k, 16) && ffb::aligned(v, 16), "%s: k and v must be 16-byte aligned", who);
   Seqs a = {const_cast<uint8_t*>(pages), page_table, row_start, ctx_len, num_pages, max_pages, B, T, HK, table_stride};
-  const int64_t items = (int64_t)T * HK, grid = (items + 2 * WARPS - 1) / (2 * WARPS);
-  FFB_REQUIRE(grid <= 0x7fffffff, "%s: T=%d HK=%d too large", who, T, HK);
-  cudaError_t e = ffb::launch(kv4_read_kernel, dim3((unsigned)grid), dim3(WARPS * 32), 0, (cudaStream_t)stream, a, k, v);
+  const dim3 grid((T + 2 * WARPS - 1) / (2 * WARPS), HK);
+  cudaError_t e = ffb::launch(kv4_read_kernel, grid, dim3(WARPS * 32), 0, (cudaStream_t)stream, a, k, v);
   if (e != cudaSuccess) return ffb::fail(FFB_ECUDA, "%s: %s", who, cudaGetErrorString(e));
   return FFB_OK;
 }
