@@ -153,12 +153,6 @@ def stream_ptr(device=None):
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def raw_stream(device):
-    """The current stream of `device` as an integer (stream_ptr without its Stream object, which
-    costs a small call more time than its launch)."""
-    return torch._C._cuda_getCurrentRawStream(device.index)
-
-
 def device_error(clear=False):
     w = c_uint32(0)
     call("ffb_device_error", ctypes.addressof(w), int(clear))

@@ -25,6 +25,8 @@ Outputs are allocated with torch on the input's device (stream-ordered, graph-sa
 through the caching allocator).  Argument errors raise ValueError (the reference uses
 assert); CUDA failures raise FFBError.  There is no CPU path.
 """
+import functools
+
 import torch
 
 from . import _lib as L
@@ -427,17 +429,28 @@ def _kv4_place(pages, page_table, row_start, ctx_len):
 
 def _kv4_call(device, name, *args):
     """`call` on `device`'s current stream, with that device current."""
+    fn = getattr(L.lib(), name)
     if torch._C._cuda_getDevice() == device.index:
-        call(name, *args, L.raw_stream(device))
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
     else:
         with torch.cuda.device(device):
-            call(name, *args, L.raw_stream(device))
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    if rc:
+        L.check(rc)
 
 
-def _kv4_out(out, shape, device):
+@functools.lru_cache(maxsize=4096)
+def _kv4_workspace(device_index, *shape):
+    """Workspace bytes of an attention call: a function of the shapes and the device alone."""
+    with torch.cuda.device(device_index):
+        return int(L.lib().ffb_attention_kv4_workspace(*shape))
+
+
+def _kv4_out(out, like, shape):
+    """`out`, checked, or a new bf16 tensor on `like`'s device (like: bf16)."""
     if out is None:
-        return torch.empty(shape, device=device, dtype=BF16)
-    _need(out.shape == shape and out.dtype == BF16 and out.is_contiguous() and out.device == device,
+        return like.new_empty(shape)
+    _need(out.shape == shape and out.dtype is BF16 and out.is_contiguous() and out.device == like.device,
           f"out must be contiguous bf16 {list(shape)}")
     return out
 
@@ -450,22 +463,24 @@ def qk_pair_kv4(qkv, qn, kn, cos, sin, pages, page_table, row_start, ctx_len, ou
     the queries [HQ, T, 128] (`out`, or a new tensor; rows of no sequence are left as they
     were).  Norm, rotation and quantisation run in one pass; the queries round once to bf16."""
     place, rows, b = _kv4_place(pages, page_table, row_start, ctx_len)
-    qw, kw = qn.weight, kn.weight
-    _bf16_cuda(qkv, qw, kw, cos, sin)
+    qw, kw, eps, dev = qn.weight, kn.weight, qn.variance_epsilon, pages.device
+    if not (qkv.dtype is qw.dtype is kw.dtype is cos.dtype is sin.dtype is BF16):
+        _need(False, "bf16 required")
+    if not (qkv.device == qw.device == kw.device == cos.device == sin.device == dev):
+        _need(False, "tensors on one device")
     _need(qkv.dim() == 2 and qkv.stride(1) == 1, "qkv [T, (HQ + 2 HK) * 128], unit last stride")
-    (t, width), hk, dev = qkv.shape, pages.shape[1], pages.device
+    (t, width), hk = qkv.shape, pages.shape[1]
     hq = width // 128 - 2 * hk
-    _need(width % 128 == 0 and hq > 0 and hq % hk == 0, "qkv width does not fit the cache's K/V heads")
-    _need(abs(qn.variance_epsilon - kn.variance_epsilon) < 1e-12, "q_norm and k_norm must share eps")
+    if width % 128 or hq <= 0 or hq % hk:
+        _need(False, f"qkv width {width} does not fit {hk} K/V heads")
+    _need(abs(eps - kn.variance_epsilon) < 1e-12, "q_norm and k_norm must share eps")
     _need(qw.shape == kw.shape == (128,) and qw.is_contiguous() and kw.is_contiguous(), "norm weights [128]")
     _need(cos.numel() == sin.numel() == t * 128 and cos.shape[-1] == sin.shape[-1] == 128, "cos, sin [T, 128]")
-    _need(qkv.device == qw.device == kw.device == cos.device == sin.device == dev, "tensors on one device")
     cos, sin = cos.contiguous(), sin.contiguous()  # held until the launch is enqueued
-    yq = _kv4_out(out, (hq, t, 128), dev)
+    yq = _kv4_out(out, qkv, (hq, t, 128))
     if t:
         _kv4_call(dev, "ffb_qk_norm_rope_kv4", qkv.data_ptr(), qkv.stride(0) if t > 1 else width, qw.data_ptr(),
-                  kw.data_ptr(), qn.variance_epsilon, cos.data_ptr(), sin.data_ptr(), yq.data_ptr(), *place, *rows, b, t,
-                  hq, hk)
+                  kw.data_ptr(), eps, cos.data_ptr(), sin.data_ptr(), yq.data_ptr(), *place, *rows, b, t, hq, hk)
     return yq
 
 
@@ -474,8 +489,7 @@ def kv4_read(pages, page_table, row_start, ctx_len, rows):
     whole sequences, pass row_start with ctx_len's running sums."""
     place, where, b = _kv4_place(pages, page_table, row_start, ctx_len)
     hk = pages.shape[1]
-    k = torch.empty((hk, rows, 128), device=pages.device, dtype=BF16)
-    v = torch.empty_like(k)
+    k, v = torch.empty((2, hk, rows, 128), device=pages.device, dtype=BF16).unbind(0)
     if rows:
         _kv4_call(pages.device, "ffb_kv4_read", *place, *where, k.data_ptr(), v.data_ptr(), b, rows, hk)
     return k, v
@@ -489,17 +503,19 @@ def attention_kv4(q, pages, page_table, row_start, ctx_len, scale, window=0, sin
     known (it sizes the launch; default T, right for any mix).  Returns [T, HQ, 128] bf16 (`out`,
     or a new tensor; rows of no sequence are left as they were)."""
     place, where, b = _kv4_place(pages, page_table, row_start, ctx_len)
-    _bf16_cuda(q)
+    dev = pages.device
+    if q.dtype is not BF16 or q.device != dev:
+        _need(False, "q must be bf16, on the cache's device")
     _need(q.dim() == 3 and q.shape[2] == 128 and q.is_contiguous(), "q must be contiguous [HQ, T, 128]")
-    (hq, t, _), hk, dev = q.shape, pages.shape[1], pages.device
-    _need(hq > 0 and hq % hk == 0, "query heads must be a multiple of the K/V heads")
-    _need(q.device == dev, "tensors on one device")
+    (hq, t, _), hk = q.shape, pages.shape[1]
+    if hq <= 0 or hq % hk:
+        _need(False, f"{hq} query heads for {hk} K/V heads")
     most = t if max_rows is None else min(max_rows, t)
     _need(most > 0 or t == 0, "max_rows must be positive")
-    y = _kv4_out(out, (t, hq, 128), dev)
+    y = _kv4_out(out, q, (t, hq, 128))
     if t:
-        need = L.lib().ffb_attention_kv4_workspace(b, t, hq, hk, most, place[4], window, sinks)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        need = _kv4_workspace(dev.index, b, t, hq, hk, most, place[4], window, sinks)
+        ws = pages.new_empty(need) if need else None
         _kv4_call(dev, "ffb_attention_kv4", q.data_ptr(), *place, *where, y.data_ptr(), ws.data_ptr() if need else None,
                   need, b, t, most, hq, hk, scale, window, sinks)
     return y
