@@ -145,8 +145,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
   uint64_t* slot_empty = slot_full + SLOTS;
   uint64_t* q_full = slot_empty + SLOTS;  // [2] per tile, as the rest
   uint64_t* s_full = q_full + 2;
-  uint64_t* p_full = s_full + 2;
-  uint64_t* o_done = p_full + 2;
+  uint64_t* p_full = s_full + 2;  // [2][2]: the first and the second page's probabilities
+  uint64_t* o_done = p_full + 4;
   uint64_t* last = o_done + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(last + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -173,7 +173,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 4);
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
+      mbar_init(&p_full[2 * i], 4);
+      mbar_init(&p_full[2 * i + 1], 4);
       mbar_init(&o_done[i], 1);
     }
     mbar_init(last, 1);
@@ -279,16 +280,24 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
         }
         __syncwarp();
       };
-      auto product = [&](int x, uint32_t u, bool first, bool free_slot) {
+      // O += P V, a page's keys as soon as their probabilities are there
+      auto product = [&](int x, uint32_t u, uint32_t parity, bool first, bool free_slot) {
         const uint64_t vd = umma_desc_sw128_mn(kvbase + (u % SLOTS) * TILE, HALF);
-        if (leader) {
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk)
-            umma_f16_ts(256 + 128 * x, 128 * x + 8 * kk, vd + kk * 2048 / 16, idesc_o, (!first || kk > 0) ? 1u : 0u);
-          umma_commit(&o_done[x]);
-          if (free_slot) umma_commit(&slot_empty[u % SLOTS]);
+        for (int half = 0; half < 2; ++half) {
+          if (!wait_uniform(&p_full[2 * x + half], parity)) return false;
+          if (leader) {
+#pragma unroll
+            for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
+              umma_f16_ts(256 + 128 * x, 128 * x + 8 * kk, vd + kk * 2048 / 16, idesc_o, (!first || kk > 0) ? 1u : 0u);
+            if (half) {
+              umma_commit(&o_done[x]);
+              if (free_slot) umma_commit(&slot_empty[u % SLOTS]);
+            }
+          }
+          __syncwarp();
         }
-        __syncwarp();
+        return true;
       };
       bool go = true;
       if (nblk > 0) {
@@ -301,18 +310,16 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
       for (int j = 0; j < nblk && go; ++j) {
         const uint32_t uv = 2 * (blk0 + j) + 1, uk = uv + 1;
         const bool more = j + 1 < nblk;
-        go = wait_slot(uv) && wait_uniform(&p_full[0], (blk0 + j) & 1u);
+        go = wait_slot(uv) && product(0, uv, (blk0 + j) & 1u, j == 0, !two);
         if (!go) break;
-        product(0, uv, j == 0, !two);
         if (more) {
           go = wait_slot(uk);
           if (!go) break;
           scores(0, uk, !two);
         }
         if (two) {
-          go = wait_uniform(&p_full[1], (blkB0 + j) & 1u);
+          go = product(1, uv, (blkB0 + j) & 1u, j == 0, true);
           if (!go) break;
-          product(1, uv, j == 0, true);
           if (more) scores(1, uk, true);
         }
       }
@@ -522,12 +529,14 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
               p[e >> 1] = pack_bf16(z.x, z.y);
             }
             tmem_st8(st + 8 * q, p);
+            if (q == 3 || q == 7) {  // a page is done: its product may start
+              tmem_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&p_full[2 * x + (q >> 2)]);
+            }
           }
           l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[x]);
         }
         if (ok && nblk > 0)
           ok = __all_sync(0xffffffffu, wait_held(&o_done[x], (base_blk + nblk - 1) & 1u, abort_flag) && !*abort_flag);
