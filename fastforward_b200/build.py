@@ -1,6 +1,6 @@
 """Builds libffb200.so in-tree (fastforward_b200/libffb200.so) with nvcc for sm_100a.
 
-Each `csrc/*.cu` compiles to a relocatable object under `fastforward_b200/_build/`
+Each `csrc/*.cu` compiles to an object (relocatable device code but for one) under `fastforward_b200/_build/`
 (rebuilt only when it or a header is newer than its object), then one nvcc call device-
 links them into the shared library.  Run `python -m fastforward_b200.build [--force]`.
 """
@@ -20,6 +20,9 @@ INCLUDE = PKG.parent / "include"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-rdc=true", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
          "-Xptxas", "-warn-spills"]
+# Units that hand registers from one warpgroup to another (setmaxnreg), which ptxas ignores in
+# relocatable code; they use no device symbol of another unit.
+WHOLE_PROGRAM = {"attention_kv4_tc.cu"}
 
 
 def nvcc():
@@ -46,7 +49,8 @@ def build(force=False, verbose=False, jobs=None):
 
     def compile_one(src):
         obj = OBJ / (src.stem + ".o")
-        cmd = [cc, *ARCH, *FLAGS, "-I", str(INCLUDE), "-c", str(src), "-o", str(obj)]
+        flags = [f.replace("-rdc=true", "-rdc=false") for f in FLAGS] if src.name in WHOLE_PROGRAM else FLAGS
+        cmd = [cc, *ARCH, *flags, "-I", str(INCLUDE), "-c", str(src), "-o", str(obj)]
         if verbose:
             cmd += ["-Xptxas", "-v"]
         r = subprocess.run(cmd, capture_output=True, text=True)

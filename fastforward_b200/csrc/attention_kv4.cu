@@ -856,56 +856,69 @@ __global__ void __launch_bounds__(THREADS, Shape<NT>::PER_SM) kv4_attention_kern
   if (tid == 0 && *abort_flag) atomicOr(&ffb_device_error_word, (uint32_t)ffb::ERR_ATTN_TIMEOUT);
 }
 
-// Joins the shares of attention_kv4_tc.cu: one warp a (row, head), its columns in the order that
-// kernel keeps them in.
+// Joins the shares of attention_kv4_tc.cu: 32 CTAs an item that was cut, one warp a column of its
+// tile, whose 128 sums lie in the order that kernel keeps them in.
 __global__ void __launch_bounds__(256) kv4_join_tc_kernel(const AttnArgs args) {
   pdl_wait();
   pdl_launch();
-  const int64_t n = (int64_t)args.seqs.T * args.HQ, at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (at >= n) return;
-  const int t = (int)(at / args.HQ), lane = threadIdx.x & 31;
-  if (t < __ldg(args.seqs.row_start) || t >= __ldg(args.seqs.row_start + args.seqs.B)) return;
+  const int cut = (int)(blockIdx.x >> 5), column = (int)(blockIdx.x & 31) * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const TcItem item = tc_item(args, cut);
+  const int G = args.HQ / args.seqs.HK, c = item.tile * 256 + column;
+  if (c >= item.rows * G) return;
   // channel d = 64 half + 8 i + g sits in column 16 g + 8 half + 2 (i % 4) + i / 4
   const int half = lane >> 4, i = (lane >> 1) & 7, col = 64 * (lane & 1) + 8 * half + 2 * (i & 3) + (i >> 2);
   Sum s = {-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
 #pragma unroll 4
   for (int p = 0; p < args.splits; ++p) {
-    const float2 ml = *reinterpret_cast<const float2*>(args.part_ml + (p * n + at) * 2);
-    const float* row = args.part_o + (p * n + at) * D + col;
+    const int64_t at = ((int64_t)cut * args.splits + p) * 256 + column;
+    const float2 ml = *reinterpret_cast<const float2*>(args.part_ml + at * 2);
+    const float* row = args.part_o + at * D + col;
     add_part(s, ml.x, ml.y, make_float4(row[0], row[16], row[32], row[48]));
   }
-  store_row(args.out + at * D, s, lane);
+  store_row(args.out + ((int64_t)(item.r0 + c / G) * args.HQ + item.kvh * G + c % G) * D, s, lane);
 }
 
 // How a call is laid out.  kernel: 1 / 2 = the register path with 8 / 16 query columns a CTA,
-// TC = the tensor-memory path with 256.  splits: TC's shares of the page axis; the register path
-// has 1 (every item one CTA's) or 0 (all pages in equal runs).
+// TC = the tensor-memory path with 256.  splits: the shares of the pages of each of TC's first
+// `cut` items, behind which come `whole` items of one CTA; the register path has 1 (every item one CTA's) or 0 (all pages in equal runs).
 constexpr int TC = 3;
 struct Plan {
-  int kernel, tiles, splits, ctas;
+  int kernel, tiles, splits, ctas, cut, whole;
   int64_t bytes;  // workspace
 };
 
-// TC's shares: enough CTAs for every SM, against the start and end of a CTA and the join.
-// step_us, cta_us: what a block of two pages and a CTA's start and end take; join_us: a share's
-// partials, written and read.
-int plan_splits(int64_t base, int64_t pages, int slots, double step_us, double cta_us, double join_us) {
-  int best = 1;
-  double best_cost = 0;
-  auto look = [&](int64_t s) {
-    if (s < 1 || s > 64 || (s > 1 && s > pages / 2)) return;  // a share has two pages at least
-    const double waves = (double)((base * s + slots - 1) / slots);
-    const double rounds = (double)((pages + 2 * s - 1) / (2 * s));
-    const double cost = waves * (rounds * step_us + cta_us) + (s > 1 ? 2.0 + join_us * s : 0.0);
-    if (best_cost == 0 || cost < best_cost) {
-      best = (int)s;
-      best_cost = cost;
+// TC: whole items while they fill every SM, the rest (or all) in shares that fill the last wave.
+// The costs in us: a block of two pages 2.4, a CTA's start and end 10, the join's launch 2, a cut
+// item's share of partial sums written and read 0.05.
+constexpr double BLOCK_US = 2.4, CTA_US = 10.0, JOIN_US = 2.0, SHARE_US = 0.05;
+void plan_tc(Plan& p, int64_t items, int64_t pages, int sms) {
+  const double item_us = (double)((pages + 1) / 2) * BLOCK_US + CTA_US;
+  double best = 0;
+  auto look = [&](int64_t whole, int64_t splits) {
+    if (splits < 1 || splits > 64 || (splits > 1 && splits > pages / 2)) return;  // a share has two pages at least
+    const int64_t shares = (items - whole) * splits;
+    const double cost = (double)(whole / sms) * item_us +
+                        (double)((shares + sms - 1) / sms) * ((double)((pages + 2 * splits - 1) / (2 * splits)) * BLOCK_US + CTA_US) +
+                        (splits > 1 ? JOIN_US + SHARE_US * (double)shares : 0.0);
+    if (best == 0 || cost < best) {
+      best = cost;
+      p.splits = (int)splits;
+      p.whole = splits > 1 ? (int)whole : (int)items;
+      p.cut = (int)items - p.whole;
     }
   };
-  for (int s = 1; s <= 4; ++s) look(s);
-  for (int wave = 1; wave <= 3; ++wave) look(wave * slots / base);  // whole waves
-  if (slots / base > pages / 2) look(pages / 2);
-  return best;
+  const int64_t full = items / sms * sms;
+  for (int64_t whole = full; whole >= 0 && whole >= full - sms; whole -= sms) {
+    if (whole == items) {
+      look(whole, 1);
+      continue;
+    }
+    for (int s = 1; s <= 4; ++s) look(whole, s);
+    for (int wave = 1; wave <= 3; ++wave) look(whole, wave * sms / (items - whole));
+    if (sms / (items - whole) > pages / 2) look(whole, pages / 2);
+  }
+  p.ctas = p.whole + p.cut * p.splits;
+  p.bytes = (int64_t)p.cut * p.splits * 256 * (D + 2) * 4;
 }
 
 Plan make_plan(int B, int T, int HQ, int HK, int max_rows, int max_pages, int window, int sinks) {
@@ -922,13 +935,13 @@ Plan make_plan(int B, int T, int HQ, int HK, int max_rows, int max_pages, int wi
   }
   const int sms = ffb::sm_count();
   if (p.kernel == TC) {
-    const double join = (double)T * HQ * (D + 2) * 4 * 2 / 5e6;  // written and read at about 5 TB/s
-    p.splits = plan_splits((int64_t)B * HK * p.tiles, pages, sms, 2.0, 6.0, join);
-    p.ctas = B * HK * p.splits;
-    p.bytes = p.splits > 1 ? (int64_t)p.splits * T * HQ * (D + 2) * 4 : 0;
+    // the tiles of all sequences: each has max_rows at most, together they have T
+    const int64_t all = (int64_t)T * (HQ / HK) / 256 + B;
+    plan_tc(p, (int64_t)HK * (all < B * tiles ? all : B * tiles), pages, sms);
   } else {
     // an item of up to two pages a warp group is done sooner than a second launch
     p.splits = pages <= 2 * GROUPS ? 1 : 0;
+    p.cut = p.whole = 0;
     p.ctas = p.splits ? B * HK : sms * (p.kernel == 1 ? Shape<1>::PER_SM : Shape<2>::PER_SM);
     p.bytes = p.splits ? 0 : (int64_t)p.ctas * 2 * (8 + width * (D + 2) * 4);
   }
@@ -957,7 +970,7 @@ cudaError_t launch_registers(const Plan& p, const AttnArgs& a, cudaStream_t st) 
 }  // namespace
 
 namespace kv4 {
-cudaError_t launch_attention_tc(const AttnArgs& a, unsigned grid_x, unsigned tiles, cudaStream_t stream);
+cudaError_t launch_attention_tc(const AttnArgs& a, unsigned ctas, cudaStream_t stream);
 }
 
 extern "C" int64_t ffb_attention_kv4_workspace(int B, int T, int HQ, int HK, int max_rows, int max_pages, int window,
@@ -986,18 +999,18 @@ extern "C" int ffb_attention_kv4(const uint16_t* q, const uint8_t* pages, int nu
   const Plan p = make_plan(B, T, HQ, HK, max_rows, max_pages, window, sinks);
   FFB_REQUIRE(p.bytes == 0 || (ws && ws_bytes >= p.bytes && ffb::aligned(ws, 16)),
               "%s: workspace of %lld bytes (16-byte aligned) needed, %lld given", who, (long long)p.bytes, (long long)ws_bytes);
-  FFB_REQUIRE((int64_t)B * HK * (p.splits > 1 ? p.splits : 1) <= 0x7fffffff, "%s: B=%d HK=%d too large", who, B, HK);
   AttnArgs a = {q, out, nullptr, 0, nullptr, nullptr,
                 {const_cast<uint8_t*>(pages), page_table, row_start, ctx_len, num_pages, max_pages, B, T, HK, table_stride},
-                HQ, p.splits, window, sinks, scale * 1.4426950408889634f};
+                HQ, p.splits, window, sinks, p.whole, p.cut, scale * 1.4426950408889634f, nullptr};
   cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e;
   if (p.kernel == TC) {
+    e = cudaGetSymbolAddress(reinterpret_cast<void**>(&a.errors), ffb_device_error_word);
+    if (e != cudaSuccess) return ffb::fail(FFB_ECUDA, "%s: %s", who, cudaGetErrorString(e));
     a.part_o = static_cast<float*>(ws);
-    a.part_ml = a.part_o + (p.splits > 1 ? (int64_t)p.splits * T * HQ * D : 0);
-    e = kv4::launch_attention_tc(a, (unsigned)p.ctas, p.tiles, st);
-    if (e == cudaSuccess && p.splits > 1)
-      e = ffb::launch(kv4_join_tc_kernel, dim3((unsigned)(((int64_t)T * HQ + 7) / 8)), dim3(256), 0, st, a);
+    a.part_ml = a.part_o + (int64_t)p.cut * p.splits * 256 * D;
+    e = kv4::launch_attention_tc(a, (unsigned)p.ctas, st);
+    if (e == cudaSuccess && p.cut > 0) e = ffb::launch(kv4_join_tc_kernel, dim3((unsigned)p.cut * 32), dim3(256), 0, st, a);
   } else {
     if (!p.splits) {  // flags, partial rows, their maxima and sums
       a.flags = static_cast<uint64_t*>(ws);

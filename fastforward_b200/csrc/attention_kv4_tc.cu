@@ -32,6 +32,11 @@ using namespace kv4;
 
 constexpr int DEQUANT = 8;              // warps
 constexpr int THREADS = 384 + 32 * DEQUANT;
+// Registers a thread by role (warps 0-3, 4-11, 12-19), out of the LAUNCH_REGS x THREADS of the launch:
+// what a role gives up, setmaxnreg.dec, the softmax takes, setmaxnreg.inc (which waits for them).
+constexpr int LAUNCH_REGS = 96, REGS_ISSUE = 88, REGS_SOFTMAX = 112, REGS_DEQUANT = 80;
+static_assert(REGS_ISSUE <= LAUNCH_REGS && REGS_DEQUANT <= LAUNCH_REGS && REGS_SOFTMAX >= LAUNCH_REGS, "wrong way");
+static_assert(128 * REGS_ISSUE + 256 * REGS_SOFTMAX + 32 * DEQUANT * REGS_DEQUANT <= LAUNCH_REGS * THREADS, "too many");
 constexpr int RAW = 6;                 // raw pages in flight
 constexpr int SLOTS = 3;               // 128-key K or V tiles
 constexpr int HALF = 128 * 128;        // 64 channels (K, Q) or columns (V) of 128 rows: 16 KB
@@ -117,21 +122,21 @@ __device__ __forceinline__ uint4 dequant8(uint32_t w, uint32_t s) {
 __device__ __forceinline__ bool not_finite2(uint32_t w) {  // either bf16 of the pair
   return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
 }
-// Named barrier over `count` threads that returns whether `pred` held in all of them.
-__device__ __forceinline__ bool all_of(int id, int count, bool pred) {
-  uint32_t out;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.b32 p, %3, 0;\n\t"
-      "barrier.cta.red.and.pred q, %1, %2, p;\n\t"
-      "selp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(out)
-      : "r"(id), "r"(count), "r"((uint32_t)pred)
-      : "memory");
-  return out != 0;
-}
 // The channel of column (chunk, pos) of O: chunk = 2 g + half holds nibbles of V's chunk g.
 __device__ __forceinline__ int nibble_of(int pos) { return (pos >> 1) | ((pos & 1) << 2); }
+
+// What a CTA does next: shared by its roles, so that it takes no registers of theirs.
+struct Work {
+  const int* table;
+  int kvh, r0, c0, clast;  // K/V head (-1: nothing more), first row, first and last column
+  int ctx, first_pos;      // tokens held; the position of the sequence's first row
+  int pos_lo, pos_hi;      // of the columns
+  int i0, i1, parts;       // its pages of ps, and how many shares those are of
+  int seen0, seen1;        // its blocks seen0 .. seen1 - 1: every column sees every key (sinks aside)
+  PageSet ps;
+  __device__ __forceinline__ int blocks() const { return (i1 - i0 + 1) / 2; }
+  __device__ __forceinline__ int page_index(int i) const { return i < ps.n_sink ? i : ps.first_page + i - ps.n_sink; }
+};
 
 __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const AttnArgs args) {
   extern __shared__ uint8_t smem_raw[];
@@ -154,11 +159,10 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
   // [16] the same of the pages of block u, two bits: what the softmax of that block masks.  It follows
   // the producer through the pages' and tiles' barriers by at most eight blocks.
   volatile int* blk_bad = raw_bad + RAW;
+  Work* work = reinterpret_cast<Work*>(smem + 2 * TILE + SLOTS * TILE + RAW * RECORD + 384);
 
   const Seqs& sv = args.seqs;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int split = blockIdx.x % args.splits;
-  const int kvh = (blockIdx.x / args.splits) % sv.HK, b = blockIdx.x / (args.splits * sv.HK);
   const int G = args.HQ / sv.HK;
 
   if (tid == 0) {
@@ -192,33 +196,71 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
   pdl_wait();
   if (tid == 0) pdl_launch();
 
-  const int r0 = min(max(__ldg(sv.row_start + b), 0), sv.T);
-  const int r1 = min(max(__ldg(sv.row_start + b + 1), r0), sv.T);
-  const int S = r1 - r0, ctx = max(__ldg(sv.ctx_len + b), 0);
-  const int ncols = S * G;
-  const int* table = sv.table + b * sv.table_stride;
-  if (ctx > sv.max_pages * PAGE && S > 0 && tid == 0) atomicOr(&ffb_device_error_word, (uint32_t)ffb::ERR_KV4_PAGE);
-
-  // Every role walks the same query tiles and blocks; the counters run over all of them.
-  uint32_t blk0 = 0;           // blocks of the tiles before this one
-  uint32_t blkB0 = 0;          // those of them that tile B took part in
-  uint32_t tiles = 0, tilesB = 0;  // tiles with blocks
+  // Every role takes the same items one after the other; its counters run over all of them.
+  uint32_t blk0 = 0;               // blocks of the items before this one
+  uint32_t blkB0 = 0;              // those of them that tile B took part in
+  uint32_t tiles = 0, tilesB = 0;  // items with blocks
   bool ok = true;
+  // The first `whole` CTAs do an item each, those behind them one of `splits` shares of the pages of
+  // an item.  If the sequences have more items than the call was laid out for, those that began an
+  // item go on with them, uncut.
+  auto find_work = [&](int step) {
+    const int share = (int)blockIdx.x - args.whole, split = share < 0 ? 0 : share % args.splits;
+    const int n = (share < 0 ? args.cut + (int)blockIdx.x : share / args.splits) + step * (args.cut + args.whole);
+    const int parts = share < 0 || step > 0 ? 1 : args.splits;
+    const TcItem item = tc_item(args, n);
+    if (lane == 0) {
+      Work w;
+      w.kvh = item.r0 < 0 || split >= parts ? -1 : item.kvh;
+      w.table = sv.table + item.b * sv.table_stride;
+      w.r0 = item.r0;
+      w.c0 = item.tile * 256;
+      w.clast = min(w.c0 + 256, item.rows * G) - 1;
+      w.ctx = item.ctx;
+      w.first_pos = item.ctx - item.rows;
+      w.pos_lo = w.first_pos + w.c0 / G;
+      w.pos_hi = w.first_pos + w.clast / G;
+      w.ps = pages_of(w.pos_lo, w.pos_hi, sv.max_pages, args.window, args.sinks);
+      const int pairs = (w.ps.n + 1) / 2;
+      w.i0 = 2 * (int)((int64_t)split * pairs / parts);
+      w.i1 = min(2 * (int)((int64_t)(split + 1) * pairs / parts), w.ps.n);
+      w.parts = parts;
+      // pages from .. to - 1 are seen whole by all columns
+      const int from = args.window > 0 ? max(w.pos_hi - args.window + PAGE, 0) / PAGE : 0;
+      const int to = min(w.pos_lo + 1, w.ps.kend) / PAGE, shift = w.ps.n_sink - w.ps.first_page - w.i0;
+      w.seen0 = (max(from + shift, w.ps.n_sink - w.i0) + 1) >> 1;
+      w.seen1 = (to + shift) >> 1;
+      *work = w;
+      if (w.ctx > sv.max_pages * PAGE) atomicOr(args.errors, (uint32_t)ffb::ERR_KV4_PAGE);
+    }
+  };
+  // Each role has a loop of its own, so that the registers of one are not those of another.
+  auto for_items = [&](auto&& before, auto&& role) {
+    for (int step = 0;; ++step) {
+      before(step);
+      __syncthreads();
+      if (work->kvh < 0) break;
+      const bool two = work->clast >= work->c0 + 128;
+      const int nblk = work->blocks();
+      role(two, nblk);
+      if (!__syncthreads_and(!*abort_flag)) break;  // all roles, or none
+      blk0 += nblk;
+      tiles += nblk > 0;
+      if (two) {
+        blkB0 += nblk;
+        tilesB += nblk > 0;
+      }
+    }
+  };
+  auto nothing = [](int) {};
 
-  for (int c0 = (int)blockIdx.y * 256; c0 < ncols && ok; c0 += (int)gridDim.y * 256) {
-    const int clast = min(c0 + 256, ncols) - 1;
-    const bool two = clast >= c0 + 128;
-    const int pos_lo = ctx - S + c0 / G, pos_hi = ctx - S + clast / G;
-    const PageSet ps = pages_of(pos_lo, pos_hi, sv.max_pages, args.window, args.sinks);
-    const int pairs = (ps.n + 1) / 2;
-    const int i0 = 2 * (int)((int64_t)split * pairs / args.splits);
-    const int i1 = min(2 * (int)((int64_t)(split + 1) * pairs / args.splits), ps.n);
-    const int nblk = (i1 - i0 + 1) / 2;
-    auto page_index = [&](int i) { return i < ps.n_sink ? i : ps.first_page + i - ps.n_sink; };
-
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_ISSUE));
+    for_items([&](int step) { if (warp == 0) find_work(step); }, [&](const bool two, const int nblk) {
     if (warp == 0) {
       // ---------------------------------------------------------------- raw pages
       if (lane == 0) {
+        const Work w = *work;
         int bad_pair = 0;
         for (int i = 0; i < 2 * nblk; ++i) {
           const uint32_t u = 2 * blk0 + i, s = u % RAW;
@@ -227,10 +269,10 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
             break;
           }
           int page = -1;
-          if (i0 + i < i1) {
-            page = __ldg(table + page_index(i0 + i));
+          if (w.i0 + i < w.i1) {
+            page = __ldg(w.table + w.page_index(w.i0 + i));
             if (page < 0 || page >= sv.num_pages) {
-              atomicOr(&ffb_device_error_word, (uint32_t)ffb::ERR_KV4_PAGE);
+              atomicOr(args.errors, (uint32_t)ffb::ERR_KV4_PAGE);
               page = -1;
             }
           }
@@ -239,7 +281,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
           if (i & 1) blk_bad[(blk0 + (i >> 1)) & 15] = bad_pair;
           if (page >= 0) {
             mbar_arrive_expect_tx(&raw_full[s], RECORD);
-            bulk_load(raw + s * RECORD, sv.pages + ((int64_t)page * sv.HK + kvh) * RECORD, RECORD, &raw_full[s]);
+            bulk_load(raw + s * RECORD, sv.pages + ((int64_t)page * sv.HK + w.kvh) * RECORD, RECORD, &raw_full[s]);
           } else {
             mbar_arrive(&raw_full[s]);
           }
@@ -324,7 +366,11 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
         }
       }
       if (!go) *abort_flag = 1;
-    } else if (warp >= 12) {
+    }
+    });
+  } else if (warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_DEQUANT));
+    for_items(nothing, [&](const bool, const int nblk) {
       // ---------------------------------------------------------------- dequantisation
       const int r8 = 8 * (warp - 12);  // this warp's eight tokens of a page
       // K: token pairs (r, r ^ 5) x four chunks meet all banks on the load and on the store;
@@ -332,6 +378,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
       const int kt = lane & 3, kr = r8 + ((lane >> 3) ^ ((lane & 4) ? 5 : 0));
       const int vk = (lane >> 1) & 3, pair = 2 * (lane >> 4) + (lane & 1);
       const int vr = r8 + ((lane & 8) ? 2 + vk : (vk < 2 ? vk : 4 + vk));
+      const Work w = *work;
       for (int j = 0; j < nblk && ok; ++j) {
         const uint32_t u = 2 * (blk0 + j);  // the K tile's number, and the first page's
         // tokens past the newest row's position are held by nobody: whatever is there is not used
@@ -340,8 +387,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
 #pragma unroll
         for (int a = 0; a < 2; ++a) {
           got = got && wait_held(&raw_full[(u + a) % RAW], ((u + a) / RAW) & 1u, abort_flag);
-          const int key0 = i0 + 2 * j + a < i1 ? page_index(i0 + 2 * j + a) * PAGE : 0;
-          live[a] = raw_bad[(u + a) % RAW] ? 0 : min(max(ps.kend - key0, 0), PAGE);
+          const int i = w.i0 + 2 * j + a, key0 = i < w.i1 ? w.page_index(i) * PAGE : 0;
+          live[a] = raw_bad[(u + a) % RAW] ? 0 : min(max(w.ps.kend - key0, 0), PAGE);
         }
 #pragma unroll
         for (int is_v = 0; is_v < 2; ++is_v) {
@@ -404,33 +451,46 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
           *abort_flag = 1;
         }
       }
-    } else if (warp >= 4) {
+    });
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
+    for_items(nothing, [&](const bool two, const int nblk) {
       // ---------------------------------------------------------------- softmax
       const int x = (warp - 4) >> 2, quarter = warp & 3, r = quarter * 32 + lane;
       if (x == 0 || two) {
         const uint32_t base_blk = x ? blkB0 : blk0;
-        const int col = c0 + 128 * x + r;
-        const bool live_row = col <= clast;
-        const int row = live_row ? r0 + col / G : 0, head = live_row ? kvh * G + col % G : 0;
-        const int pos = live_row ? ctx - S + col / G : -1;
+        const volatile Work& w = *work;
         const float sc = fmaxf(fabsf(args.scale_log2), 1e-37f);  // scale 0: a masked -inf stays one
+        // this thread's column (past the last: the last one's), and its row and head, which shuffles
+        // hand on
+        auto column = [&] { return min(w.c0 + 128 * x + r, w.clast); };
+        auto place_of = [&] { return w.r0 + column() / G; };
+        auto head_of = [&] { return w.kvh * G + column() % G; };
         // this warp's 32 rows of Q, negated for a negative scale (exact), eight channels a chunk in
-        // the order 0 4 1 5 2 6 3 7; sixteen lanes copy one row.  A tile without blocks has no queries:
-        // no product would keep its warps from staging output over rows that others still write
+        // the order 0 4 1 5 2 6 3 7; sixteen lanes copy one row, eight loads in flight.  A tile without
+        // blocks has no queries: no product would keep its warps from staging output over rows that
+        // others still write
         if (nblk > 0) {
           const uint32_t flip = args.scale_log2 < 0.f ? 0x80008000u : 0u;
+          const int ch = lane & 15, place = place_of(), head = head_of();
 #pragma unroll
-          for (int k = 0; k < 32; k += 2) {
-            const int rr = quarter * 32 + k + (lane >> 4), cc = c0 + 128 * x + rr, ch = lane & 15;
-            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-            if (cc <= clast)
-              v = __ldg(reinterpret_cast<const uint4*>(
-                  args.q + ((int64_t)(kvh * G + cc % G) * sv.T + r0 + cc / G) * D + 8 * ch));
-            // channels 8 ch .. of group ch / 4: chunk 4 (j & 1) + t of half j / 2 with j = ch / 4, t = ch % 4
-            const uint4 y = make_uint4(__byte_perm(v.x, v.z, 0x5410) ^ flip, __byte_perm(v.x, v.z, 0x7632) ^ flip,
-                                       __byte_perm(v.y, v.w, 0x5410) ^ flip, __byte_perm(v.y, v.w, 0x7632) ^ flip);
-            const int chunk = ch & 7;
-            *reinterpret_cast<uint4*>(sq + x * TILE + (ch >> 3) * HALF + rr * 128 + ((chunk ^ (rr & 7)) << 4)) = y;
+          for (int k0 = 0; k0 < 32; k0 += 16) {
+            uint4 in[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const int from = k0 + 2 * k + (lane >> 4);
+              const int64_t at = (int64_t)__shfl_sync(0xffffffffu, head, from) * sv.T + __shfl_sync(0xffffffffu, place, from);
+              in[k] = __ldg(reinterpret_cast<const uint4*>(args.q + at * D + 8 * ch));
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const int rr = quarter * 32 + k0 + 2 * k + (lane >> 4);
+              const uint4 v = w.c0 + 128 * x + rr <= w.clast ? in[k] : make_uint4(0u, 0u, 0u, 0u);
+              // channels 8 ch .. of group ch / 4: chunk 4 (j & 1) + t of half j / 2 with j = ch / 4, t = ch % 4
+              const uint4 y = make_uint4(__byte_perm(v.x, v.z, 0x5410) ^ flip, __byte_perm(v.x, v.z, 0x7632) ^ flip,
+                                         __byte_perm(v.y, v.w, 0x5410) ^ flip, __byte_perm(v.y, v.w, 0x7632) ^ flip);
+              *reinterpret_cast<uint4*>(sq + x * TILE + (ch >> 3) * HALF + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4)) = y;
+            }
           }
           fence_proxy_async_smem();
           __syncwarp();
@@ -441,23 +501,24 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
         float m = -INFINITY, neg = 0.f, l = 0.f;  // neg: -m, 0 while nothing has been seen
         const float2 sc2 = make_float2(sc, sc);
         for (int j = 0; j < nblk; ++j) {
+          const bool part = j < w.seen0 || j >= w.seen1;
           if (!__all_sync(0xffffffffu, wait_held(&s_full[x], (base_blk + j) & 1u, abort_flag) && !*abort_flag)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const int ia = i0 + 2 * j, bad = blk_bad[(blk0 + j) & 15];
-          const int ka = page_index(ia) * PAGE, kb = page_index(ia + 1) * PAGE;
-          auto seen_by_all = [&](int key0) {
-            return key0 + PAGE - 1 <= pos_lo && key0 + PAGE <= ps.kend &&
-                   (args.window == 0 || pos_hi - key0 < args.window || key0 + PAGE <= args.sinks);
-          };
-          const bool whole = bad == 0 && seen_by_all(ka) && seen_by_all(kb);
-          // columns of this row that count, per page: c <= hi and (c >= lo or c < sk)
-          const int top = min(pos, ps.kend - 1), low = args.window > 0 ? pos - args.window + 1 : 0;
-          if (!whole) {  // rare blocks: the scores that do not count become -inf where they lie
-            const int hi[2] = {(bad & 1) ? -1 : top - ka, (bad & 2) ? -1 : top - kb};
-            const int lo[2] = {low - ka, low - kb}, sk[2] = {args.sinks - ka, args.sinks - kb};
+          const int bad = blk_bad[(blk0 + j) & 15];
+          if (part || bad) {  // rare blocks: the scores that do not count become -inf where they lie
+            const int ia = w.i0 + 2 * j;
+            int key0[2];
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+              key0[a] = (ia + a < w.ps.n_sink ? ia + a : w.ps.first_page + ia + a - w.ps.n_sink) * PAGE;
+            // the keys of a page that this column sees: c <= hi and (c >= lo or c < sk)
+            const int pos = w.first_pos + column() / G;
+            const int top = min(pos, w.ps.kend - 1), low = args.window > 0 ? pos - args.window + 1 : 0;
+            const int hi[2] = {(bad & 1) ? -1 : top - key0[0], (bad & 2) ? -1 : top - key0[1]};
+            const int lo[2] = {low - key0[0], low - key0[1]}, sk[2] = {args.sinks - key0[0], args.sinks - key0[1]};
 #pragma unroll 1
             for (int q = 0; q < 8; ++q) {
               const int first = 16 * (q & 3), h = hi[q >> 2] - first, l0 = lo[q >> 2] - first, s0 = sk[q >> 2] - first;
@@ -473,15 +534,15 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
             tmem_wait_st();
           }
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-          uint32_t v[2][32];
-          tmem_ld32_async(st, v[0]);
+          uint32_t v[2][16];
+          tmem_ld16_async(st, v[0]);
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
+          for (int q = 0; q < 8; ++q) {
             tmem_wait_ld();
             reg_fence(v[q & 1]);
-            if (q < 3) tmem_ld32_async(st + 32 * (q + 1), v[(q + 1) & 1]);
+            if (q < 7) tmem_ld16_async(st + 16 * (q + 1), v[(q + 1) & 1]);
 #pragma unroll
-            for (int e = 0; e < 32; e += 2)
+            for (int e = 0; e < 16; e += 2)
               mx[(e >> 1) & 3] = fmaxf(mx[(e >> 1) & 3], fmaxf(__uint_as_float(v[q & 1][e]), __uint_as_float(v[q & 1][e + 1])));
           }
           uint32_t w[2][16];  // the scores again, for the probabilities: on their way while the maximum is looked at
@@ -543,10 +604,10 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
         if (!ok) *abort_flag = 1;
         if (ok) {
           tc_fence_after();
-          const int64_t at = (int64_t)row * args.HQ + head;
-          if (args.splits > 1) {
-            // fp32 partials in the columns' order; kv4_combine takes them back to channels
-            const int64_t pt = (int64_t)split * sv.T * args.HQ + at;
+          if (w.parts > 1) {
+            // fp32 partials in the columns' order; kv4_join_tc_kernel takes them back to channels
+            const int64_t pt = (int64_t)((int)blockIdx.x - args.whole) * 256 + 128 * x + r;
+            const bool live_row = w.c0 + 128 * x + r <= w.clast;
             if (live_row) *reinterpret_cast<float2*>(args.part_ml + pt * 2) = make_float2(m, l);
 #pragma unroll 1
             for (int q = 0; q < 8; ++q) {
@@ -588,29 +649,21 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
               }
             }
             __syncwarp();
-            for (int k = 0; k < 32; ++k) {
-              const int rr = quarter * 32 + k, cc = c0 + 128 * x + rr;
-              if (cc > clast) break;
-              const uint32_t* src = reinterpret_cast<const uint32_t*>(sq + x * TILE) + rr * 64;
-              uint32_t* dst = reinterpret_cast<uint32_t*>(args.out + ((int64_t)(r0 + cc / G) * args.HQ + kvh * G + cc % G) * D);
-              dst[lane] = src[lane ^ k];
-              dst[32 + lane] = src[32 + (lane ^ k)];
+            const uint32_t* src = reinterpret_cast<const uint32_t*>(sq + x * TILE) + quarter * 32 * 64;
+            const int place = place_of(), head = head_of(), n = min(w.clast - (w.c0 + 128 * x + quarter * 32) + 1, 32);
+#pragma unroll 8
+            for (int k = 0; k < n; ++k) {
+              uint32_t* dst = reinterpret_cast<uint32_t*>(args.out) +
+                              ((int64_t)__shfl_sync(0xffffffffu, place, k) * args.HQ + __shfl_sync(0xffffffffu, head, k)) * 64;
+              dst[lane] = src[64 * k + (lane ^ k)];
+              dst[32 + lane] = src[64 * k + 32 + (lane ^ k)];
             }
             __syncwarp();
           }
           tc_fence_before();
         }
-        // the four warps of a tile go on together (their staged rows and the next queries share the
-        // Q tile) and with one verdict, or leave together
-        ok = all_of(1 + x, 128, ok && !*abort_flag);
       }
-    }
-    blk0 += nblk;
-    tiles += nblk > 0;
-    if (two) {
-      blkB0 += nblk;
-      tilesB += nblk > 0;
-    }
+    });
   }
 
   if (warp == 1) {
@@ -625,7 +678,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
   }
   tc_fence_before();
   __syncthreads();
-  if (tid == 0 && *abort_flag) atomicOr(&ffb_device_error_word, (uint32_t)ffb::ERR_ATTN_TIMEOUT);
+  if (tid == 0 && *abort_flag) atomicOr(args.errors, (uint32_t)ffb::ERR_ATTN_TIMEOUT);
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
@@ -636,10 +689,16 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
 }  // namespace
 
 namespace kv4 {
-cudaError_t launch_attention_tc(const AttnArgs& a, unsigned grid_x, unsigned tiles, cudaStream_t stream) {
+cudaError_t launch_attention_tc(const AttnArgs& a, unsigned ctas, cudaStream_t stream) {
+  // setmaxnreg is right for one number of registers at the launch alone
+  static const int launch_regs = [] {
+    cudaFuncAttributes f;
+    return cudaFuncGetAttributes(&f, kv4_attention_tc_kernel) == cudaSuccess ? f.numRegs : 0;
+  }();
+  if (launch_regs != LAUNCH_REGS) return cudaErrorInvalidKernelImage;
   cudaError_t e = ffb::set_smem_attr(reinterpret_cast<const void*>(kv4_attention_tc_kernel), SMEM);
   if (e == cudaSuccess)
-    e = ffb::launch(kv4_attention_tc_kernel, dim3(grid_x, tiles), dim3(THREADS), SMEM, stream, a);
+    e = ffb::launch(kv4_attention_tc_kernel, dim3(ctas), dim3(THREADS), SMEM, stream, a);
   return e;
 }
 }  // namespace kv4

@@ -61,7 +61,9 @@ int ensure_silu_table(cudaStream_t stream);
 }  // namespace ffb
 
 // One error word per device that loads the library.
+#ifdef __CUDACC_RDC__  // a unit compiled on its own gets the word's address as an argument
 extern __device__ uint32_t ffb_device_error_word;
+#endif
 
 // ------------------------------------------------------------------ numeric helpers
 __device__ __forceinline__ float bf2f(uint16_t b) { return __uint_as_float(uint32_t(b) << 16); }

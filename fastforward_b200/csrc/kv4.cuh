@@ -65,12 +65,49 @@ struct AttnArgs {
   uint16_t* out;      // [T, HQ, 128]
   uint64_t* flags;    // [CTAs][2]: `tag` once that part is written (register path, equal runs)
   uint64_t tag;
-  float* part_o;      // partial rows of 128, relative to their maxima: register path [CTAs][2][columns], TC [splits][T * HQ]
+  float* part_o;      // partial rows of 128, relative to their maxima: register path [CTAs][2][columns], TC [cut][splits][256]
   float* part_ml;     // their (maximum, sum) pairs
   Seqs seqs;
   int HQ, splits, window, sinks;
+  int whole, cut;  // TC: items that one CTA does, and before them those in `splits` shares
   float scale_log2;
+  uint32_t* errors;  // TC: the device's error word
 };
+
+// The TC path's items: 256 columns ((row, head of the group) pairs) of a K/V head of a sequence,
+// numbered sequence by sequence, tile by tile, the heads of a tile next to each other.  Found by a
+// converged warp, 32 sequences a step; r0 = -1 behind the last item.
+struct TcItem {
+  int b, kvh, tile, r0, rows, ctx;
+};
+__device__ __forceinline__ TcItem tc_item(const AttnArgs& a, int item) {
+  const Seqs& sv = a.seqs;
+  const int lane = threadIdx.x & 31, G = a.HQ / sv.HK, kvh = item % sv.HK;
+  int t = item / sv.HK;
+  for (int b0 = 0; b0 < sv.B; b0 += 32) {
+    const int b = b0 + lane;
+    int r0 = 0, rows = 0, ctx = 0;
+    if (b < sv.B) {
+      ctx = max(__ldg(sv.ctx_len + b), 0);
+      r0 = min(max(__ldg(sv.row_start + b), 0), sv.T);
+      rows = min(max(__ldg(sv.row_start + b + 1), r0), sv.T) - r0;
+    }
+    const int tiles = (rows * G + 255) >> 8;
+    int sum = tiles;  // of the lanes up to this one
+    for (int d = 1; d < 32; d <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += other;
+    }
+    const uint32_t in = __ballot_sync(0xffffffffu, sum > t);
+    if (in) {
+      const int src = __ffs(in) - 1;
+      return {b0 + src, kvh, __shfl_sync(0xffffffffu, t - sum + tiles, src), __shfl_sync(0xffffffffu, r0, src),
+              __shfl_sync(0xffffffffu, rows, src), __shfl_sync(0xffffffffu, ctx, src)};
+    }
+    t -= __shfl_sync(0xffffffffu, sum, 31);
+  }
+  return {0, 0, 0, -1, 0, 0};
+}
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
