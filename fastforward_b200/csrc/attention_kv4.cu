@@ -856,26 +856,45 @@ __global__ void __launch_bounds__(THREADS, Shape<NT>::PER_SM) kv4_attention_kern
   if (tid == 0 && *abort_flag) atomicOr(&ffb_device_error_word, (uint32_t)ffb::ERR_ATTN_TIMEOUT);
 }
 
-// Joins the shares of attention_kv4_tc.cu: 32 CTAs an item that was cut, one warp a column of its
-// tile, whose 128 sums lie in the order that kernel keeps them in.
+// Joins the shares of attention_kv4_tc.cu: 16 CTAs an item that was cut, 32 rows and 64 channels each.
+// Channel 64 half + 8 i + g of a row sits in column 16 g + 8 half + 2 (i % 4) + i / 4 of its sums, and
+// columns 4 k .. 4 k + 3 of all 256 rows lie next to each other: warp g takes k = 4 g + 2 half and the
+// next, a lane a row, and the rows leave through shared memory.
 __global__ void __launch_bounds__(256) kv4_join_tc_kernel(const AttnArgs args) {
+  __shared__ uint16_t sh[32][66];
   pdl_wait();
   pdl_launch();
-  const int cut = (int)(blockIdx.x >> 5), column = (int)(blockIdx.x & 31) * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int cut = (int)(blockIdx.x >> 4), first = (int)(blockIdx.x >> 1 & 7) * 32, half = (int)(blockIdx.x & 1);
+  const int g = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const TcItem item = tc_item(args, cut);
-  const int G = args.HQ / args.seqs.HK, c = item.tile * 256 + column;
-  if (c >= item.rows * G) return;
-  // channel d = 64 half + 8 i + g sits in column 16 g + 8 half + 2 (i % 4) + i / 4
-  const int half = lane >> 4, i = (lane >> 1) & 7, col = 64 * (lane & 1) + 8 * half + 2 * (i & 3) + (i >> 2);
-  Sum s = {-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+  const int G = args.HQ / args.seqs.HK, c0 = item.tile * 256 + first, n = min(item.rows * G - c0, 32);  // rows here
+  if (n <= 0) return;
+  const int row = first + min(lane, n - 1);
+  Sum s[2];
+  for (int e = 0; e < 2; ++e) s[e] = {-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
 #pragma unroll 4
   for (int p = 0; p < args.splits; ++p) {
-    const int64_t at = ((int64_t)cut * args.splits + p) * 256 + column;
-    const float2 ml = *reinterpret_cast<const float2*>(args.part_ml + at * 2);
-    const float* row = args.part_o + at * D + col;
-    add_part(s, ml.x, ml.y, make_float4(row[0], row[16], row[32], row[48]));
+    const int64_t part = (int64_t)cut * args.splits + p;
+    const float2 ml = *reinterpret_cast<const float2*>(args.part_ml + (part * 256 + row) * 2);
+    const float4* from = reinterpret_cast<const float4*>(args.part_o) + (part * (D / 4) + 4 * g + 2 * half) * 256 + row;
+    const float4 v0 = from[0], v1 = from[256];
+    add_part(s[0], ml.x, ml.y, v0);
+    add_part(s[1], ml.x, ml.y, v1);
   }
-  store_row(args.out + ((int64_t)(item.r0 + c / G) * args.HQ + item.kvh * G + c % G) * D, s, lane);
+  const float r = s[0].l == 0.f ? 0.f : 1.f / s[0].l;
+  for (int e = 0; e < 2; ++e) {  // columns 4 e .. of eight: i = 2 e, 2 e + 4, 2 e + 1, 2 e + 5
+    const uint32_t lo = pack_bf16(s[e].o.x * r, s[e].o.y * r), hi = pack_bf16(s[e].o.z * r, s[e].o.w * r);
+    sh[lane][8 * (2 * e) + g] = (uint16_t)lo;
+    sh[lane][8 * (2 * e + 4) + g] = (uint16_t)(lo >> 16);
+    sh[lane][8 * (2 * e + 1) + g] = (uint16_t)hi;
+    sh[lane][8 * (2 * e + 5) + g] = (uint16_t)(hi >> 16);
+  }
+  __syncthreads();
+  for (int k = g; k < n; k += 8) {
+    const int c = c0 + k;
+    uint32_t* to = reinterpret_cast<uint32_t*>(args.out + ((int64_t)(item.r0 + c / G) * args.HQ + item.kvh * G + c % G) * D);
+    to[32 * half + lane] = *reinterpret_cast<const uint32_t*>(&sh[k][2 * lane]);
+  }
 }
 
 // How a call is laid out.  kernel: 1 / 2 = the register path with 8 / 16 query columns a CTA,
@@ -888,17 +907,18 @@ struct Plan {
 };
 
 // TC: whole items while they fill every SM, the rest (or all) in shares that fill the last wave.
-// The costs in us: a block of two pages 2.4, a CTA's start and end 10, the join's launch 2, a cut
-// item's share of partial sums written and read 0.05.
-constexpr double BLOCK_US = 2.4, CTA_US = 10.0, JOIN_US = 2.0, SHARE_US = 0.05;
+// The costs in us: a block of two pages 2.2, a CTA's start and end 10, the join's launch 2, a cut
+// item's share of partial sums written and read 0.07.
+constexpr double BLOCK_US = 2.2, CTA_US = 10.0, JOIN_US = 2.0, SHARE_US = 0.07;
 void plan_tc(Plan& p, int64_t items, int64_t pages, int sms) {
-  const double item_us = (double)((pages + 1) / 2) * BLOCK_US + CTA_US;
+  const int64_t blocks = (pages + 1) / 2;
+  const double item_us = (double)blocks * BLOCK_US + CTA_US;
   double best = 0;
   auto look = [&](int64_t whole, int64_t splits) {
-    if (splits < 1 || splits > 64 || (splits > 1 && splits > pages / 2)) return;  // a share has two pages at least
+    if (splits < 1 || splits > 64 || (splits > 1 && splits > blocks)) return;
     const int64_t shares = (items - whole) * splits;
     const double cost = (double)(whole / sms) * item_us +
-                        (double)((shares + sms - 1) / sms) * ((double)((pages + 2 * splits - 1) / (2 * splits)) * BLOCK_US + CTA_US) +
+                        (double)((shares + sms - 1) / sms) * ((double)((blocks + splits - 1) / splits) * BLOCK_US + CTA_US) +
                         (splits > 1 ? JOIN_US + SHARE_US * (double)shares : 0.0);
     if (best == 0 || cost < best) {
       best = cost;
@@ -909,13 +929,10 @@ void plan_tc(Plan& p, int64_t items, int64_t pages, int sms) {
   };
   const int64_t full = items / sms * sms;
   for (int64_t whole = full; whole >= 0 && whole >= full - sms; whole -= sms) {
-    if (whole == items) {
-      look(whole, 1);
-      continue;
-    }
-    for (int s = 1; s <= 4; ++s) look(whole, s);
+    look(whole, 1);
+    if (whole == items) continue;
     for (int wave = 1; wave <= 3; ++wave) look(whole, wave * sms / (items - whole));
-    if (sms / (items - whole) > pages / 2) look(whole, pages / 2);
+    for (int64_t n = 1; n <= 6; ++n) look(whole, (blocks + n - 1) / n);  // shares of n blocks
   }
   p.ctas = p.whole + p.cut * p.splits;
   p.bytes = (int64_t)p.cut * p.splits * 256 * (D + 2) * 4;
@@ -1010,7 +1027,7 @@ extern "C" int ffb_attention_kv4(const uint16_t* q, const uint8_t* pages, int nu
     a.part_o = static_cast<float*>(ws);
     a.part_ml = a.part_o + (int64_t)p.cut * p.splits * 256 * D;
     e = kv4::launch_attention_tc(a, (unsigned)p.ctas, st);
-    if (e == cudaSuccess && p.cut > 0) e = ffb::launch(kv4_join_tc_kernel, dim3((unsigned)p.cut * 32), dim3(256), 0, st, a);
+    if (e == cudaSuccess && p.cut > 0) e = ffb::launch(kv4_join_tc_kernel, dim3((unsigned)p.cut * 16), dim3(256), 0, st, a);
   } else {
     if (!p.splits) {  // flags, partial rows, their maxima and sums
       a.flags = static_cast<uint64_t*>(ws);

@@ -605,26 +605,29 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
         if (ok) {
           tc_fence_after();
           if (w.parts > 1) {
-            // fp32 partials in the columns' order; kv4_join_tc_kernel takes them back to channels
-            const int64_t pt = (int64_t)((int)blockIdx.x - args.whole) * 256 + 128 * x + r;
-            const bool live_row = w.c0 + 128 * x + r <= w.clast;
-            if (live_row) *reinterpret_cast<float2*>(args.part_ml + pt * 2) = make_float2(m, l);
+            // fp32 sums in the columns' order, four columns of all 256 rows next to each other, so that a
+            // warp stores 512 bytes in a row; kv4_join_tc_kernel takes them back to channels
+            const int64_t part = (int64_t)blockIdx.x - args.whole;
+            const int column = 128 * x + r;
+            const bool live_row = w.c0 + column <= w.clast;
+            float4* to = reinterpret_cast<float4*>(args.part_o) + part * (256 * D / 4) + column;
+            if (live_row) *reinterpret_cast<float2*>(args.part_ml + (part * 256 + column) * 2) = make_float2(m, l);
 #pragma unroll 1
-            for (int q = 0; q < 8; ++q) {
-              uint32_t v[16];
+            for (int q = 0; q < 4; ++q) {
+              uint32_t v[32];
               if (nblk > 0) {
-                tmem_ld16_async(ot + 16 * q, v);
+                tmem_ld32_async(ot + 32 * q, v);
                 tmem_wait_ld();
                 reg_fence(v);
               } else {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) v[e] = 0u;
+                for (int e = 0; e < 32; ++e) v[e] = 0u;
               }
               if (live_row)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  *reinterpret_cast<uint4*>(args.part_o + pt * D + 16 * q + 4 * e) =
-                      make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+                for (int e = 0; e < 8; ++e)
+                  to[256 * (8 * q + e)] = make_float4(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1]),
+                                                      __uint_as_float(v[4 * e + 2]), __uint_as_float(v[4 * e + 3]));
             }
           } else {
             // rows staged over this warp's part of the Q tile (every S product has been read), words
