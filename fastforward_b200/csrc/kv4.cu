@@ -11,11 +11,9 @@
 // issued together), the last its key and value heads.
 //
 // The codes are those of the formula in exact arithmetic, up to fp64's rounding: a key next to
-// the border of two codes must not fall to either side by chance.  x w is exact in fp32 (two
-// bf16), so is its product with the bf16 cosine (24 bits); only the difference of the two
-// products and the norm's factor are fp64.  Everything after that is fp32, with the distance to
-// the next border looked at, and done again in fp64 where that distance is within fp32's error
-// (about one head in a thousand).  Values are bf16: x - q s is exact, so borders are seen as such.
+// the border of two codes must not fall to either side by chance.  Keys are worked out in fp32 with
+// a bound on the error, and again in fp64 where a value lies within it of a border (about one head in
+// 200).  Values are bf16: x - q s is exact, so borders are seen as such.
 #include "kv4.cuh"
 #include "pdl.cuh"
 
@@ -39,13 +37,6 @@ __device__ __forceinline__ double up5(double v) {
 __device__ __forceinline__ float up5(float v) {
   const uint32_t b = __float_as_uint(v), low = (1u << 19) - 1;
   return __uint_as_float((b + low) & ~low);
-}
-// (int) code of x under the scale s = 1 / r from t = x r: the nearest integer, and whether t lies too
-// near the border of two for fp32 to tell.
-__device__ __forceinline__ int code_of(float t, bool& close) {
-  const float q = rintf(t);
-  close |= fabsf(fabsf(t - q) - 0.5f) < 4e-6f;  // |t| <= 7: y r is within 3 x 2^-24 x 7 of the quotient
-  return (int)fminf(fmaxf(q, -7.f), 7.f);
 }
 __device__ __forceinline__ float group_max(float top, uint32_t mask) {
 #pragma unroll
@@ -80,40 +71,44 @@ __device__ __forceinline__ uint32_t value_codes(const float (&y)[4], uint32_t ma
   }
   return codes;
 }
-// Keys: fp64.
-__device__ __forceinline__ uint32_t key_codes(const double (&y)[4], uint32_t mask, float& scale) {
-  float f[4], top = 0.f;
+// Keys, in fp32: y is within 9.5 x 2^-24 of the formula's value, so a quotient y / s <= 7 within
+// 11.5 x 2^-24 x 7 < 1e-5 and max / 7 within 10.5 units of its last place.  `doubt`: fp32 cannot tell on
+// which side of a border a value lies, or the group's range is not its own.
+__device__ __forceinline__ uint32_t key_codes(const float (&d)[4], float inv, uint32_t mask, float& scale, bool& doubt) {
+  float top = 0.f;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    f[e] = (float)y[e];
-    top = fabsf(f[e]) < BIG ? fmaxf(top, fabsf(f[e])) : INFINITY;
-  }
+  for (int e = 0; e < 4; ++e) top = fabsf(d[e]) < 1e36f ? fmaxf(top, fabsf(d[e])) : INFINITY;
   top = group_max(top, mask);
-  if (!(top < BIG) || top < SMALL) {
-    scale = top < BIG ? 0.f : __uint_as_float(0x7fc00000u);
-    return 0x8888u;
-  }
-  const float seventh = __fdiv_rn(top, 7.f);
-  float s = up5(seventh);
-  const uint32_t low = (__float_as_uint(seventh) + 8u) & ((1u << 19) - 1);
-  bool close = low < 16u;  // within 8 units of a number of five bits
+  const float most = top * inv, seventh = __fdiv_rn(most, 7.f), s = up5(seventh);
+  doubt |= !(top > 1e-30f && top < 1e36f && most > 1e-29f && most < 1e37f) ||
+           ((__float_as_uint(seventh) + 16u) & ((1u << 19) - 1)) < 32u;
   const float r = __frcp_rn(s);
+  scale = s;
   uint32_t codes = 0;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) codes |= (uint32_t)(code_of(f[e] * r, close) + 8) << (4 * e);
-  if (__any_sync(mask, close)) {  // in fp64
-    double most = 0.0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) most = fmax(most, fabs(y[e]));
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) most = fmax(most, __shfl_xor_sync(mask, most, o));
-    const double exact = up5(most / 7.0);
-    s = (float)exact;
-    codes = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) codes |= (uint32_t)((int)fmin(fmax(rint(y[e] / exact), -7.0), 7.0) + 8) << (4 * e);
+  for (int e = 0; e < 4; ++e) {
+    const float t = d[e] * inv * r, q = rintf(t);
+    doubt |= fabsf(fabsf(t - q) - 0.5f) < 1e-5f;
+    codes |= (uint32_t)((int)fminf(fmaxf(q, -7.f), 7.f) + 8) << (4 * e);
   }
-  scale = s;
+  return codes;
+}
+// Keys, in fp64: the formula as it stands.
+__device__ __forceinline__ uint32_t key_codes(const double (&y)[4], uint32_t mask, float& scale) {
+  double top = 0.0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) top = fabs(y[e]) < (double)BIG ? fmax(top, fabs(y[e])) : (double)INFINITY;
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) top = fmax(top, __shfl_xor_sync(mask, top, o));
+  if (!(top < (double)BIG) || top < (double)SMALL) {
+    scale = top < (double)BIG ? 0.f : __uint_as_float(0x7fc00000u);
+    return 0x8888u;
+  }
+  const double s = up5(top / 7.0);
+  scale = (float)s;
+  uint32_t codes = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) codes |= (uint32_t)((int)fmin(fmax(rint(y[e] / s), -7.0), 7.0) + 8) << (4 * e);
   return codes;
 }
 
@@ -184,17 +179,59 @@ __device__ __forceinline__ void load_turn(const WriteArgs& p, int t, int i, Turn
   unpack4(__ldg(reinterpret_cast<const uint2*>(p.sin + at + 64)), r.sb);
 }
 
+// The codes of one key, lane i's low and high ones, and the scales of its two groups.
+struct KeyCodes {
+  uint32_t lo, hi;
+  float s_lo, s_hi;
+};
+// In fp64, from the inputs.
+__device__ __forceinline__ KeyCodes exact_key(const uint2* x, const uint2* w, const uint2* c, const uint2* s, float eps, int i,
+                                           uint32_t mask) {
+  float xa[4], xb[4], wa[4], wb[4], ca[4], cb[4], sa[4], sb[4];
+  unpack4(__ldg(x + i), xa);
+  unpack4(__ldg(x + 16 + i), xb);
+  unpack4(__ldg(w + i), wa);
+  unpack4(__ldg(w + 16 + i), wb);
+  unpack4(__ldg(c + i), ca);
+  unpack4(__ldg(c + 16 + i), cb);
+  unpack4(__ldg(s + i), sa);
+  unpack4(__ldg(s + 16 + i), sb);
+  double sum = 0.0, ya[4], yb[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) sum += (double)xa[e] * (double)xa[e] + (double)xb[e] * (double)xb[e];
+  const double norm = 1.0 / sqrt(head_sum(sum, mask) / D + (double)eps);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const double na = (double)xa[e] * norm * (double)wa[e], nb = (double)xb[e] * norm * (double)wb[e];
+    ya[e] = na * (double)ca[e] - nb * (double)sa[e];
+    yb[e] = nb * (double)cb[e] + na * (double)sb[e];
+  }
+  KeyCodes k;
+  k.lo = key_codes(ya, mask, k.s_lo);
+  k.hi = key_codes(yb, mask, k.s_hi);
+  return k;
+}
+
+// Called, it takes no registers of the common path: a fifth CTA an SM for long calls (7128 rows of 64 + 8
+// heads: 74.6 -> 70.5 us).  Where every CTA is resident anyway it is inline (320 rows: 6.9 -> 6.4 us).
+__device__ __noinline__ KeyCodes exact_key_call(const uint2* x, const uint2* w, const uint2* c, const uint2* s, float eps,
+                                                int i, uint32_t mask) {
+  return exact_key(x, w, c, s, eps, i, mask);
+}
+
 // U: query heads of a half warp.
 template <int U>
-__global__ void __launch_bounds__(WARPS * 32, 4) kv4_write_kernel(const WriteArgs p, int q_chunks) {
+__global__ void __launch_bounds__(WARPS * 32, U > 1 ? 5 : 4) kv4_write_kernel(const WriteArgs p, int q_chunks) {
   pdl_wait();
   pdl_launch();
-  const int lane = threadIdx.x & 31, i = lane & 15, slot = threadIdx.x >> 4, t = blockIdx.x;
+  const int lane = threadIdx.x & 31, i = lane & 15, slot = threadIdx.x >> 4;
+  const int t = (int)(blockIdx.z * gridDim.y + blockIdx.y), chunk = (int)blockIdx.x;  // a row's CTAs next to each other
+  if (t >= p.seqs.T) return;
   const uint32_t mask = 0xffffu << (lane & 16);
   const int HK = p.seqs.HK;
-  const uint16_t* x = p.qkv + t * p.row_stride + 4 * i;
-  if ((int)blockIdx.y < q_chunks) {
-    const int h0 = (blockIdx.y * 2 * WARPS + slot) * U;
+  const uint16_t* x = p.qkv + (int64_t)t * p.row_stride + 4 * i;
+  if (chunk < q_chunks) {
+    const int h0 = (chunk * 2 * WARPS + slot) * U;
     uint2 ua[U], ub[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -232,7 +269,7 @@ __global__ void __launch_bounds__(WARPS * 32, 4) kv4_write_kernel(const WriteArg
     }
     return;
   }
-  const int pair = (blockIdx.y - q_chunks) * 2 * WARPS + slot;
+  const int pair = (chunk - q_chunks) * 2 * WARPS + slot;
   if (pair >= 2 * HK) return;
   const bool is_v = pair >= HK;
   const int h = is_v ? pair - HK : pair;
@@ -256,31 +293,32 @@ __global__ void __launch_bounds__(WARPS * 32, 4) kv4_write_kernel(const WriteArg
   } else {
     Turn r;
     load_turn(p, t, i, r);
-    float wa[4], wb[4];
+    float wa[4], wb[4], ss = 0.f, da[4], db[4];
     unpack4(__ldg(reinterpret_cast<const uint2*>(p.k_norm + 4 * i)), wa);
     unpack4(__ldg(reinterpret_cast<const uint2*>(p.k_norm + 64 + 4 * i)), wb);
-    double ss = 0.0;  // bf16 squares are exact in fp32, their fp64 sum does not depend on its order
 #pragma unroll
-    for (int e = 0; e < 4; ++e) ss += (double)(xa[e] * xa[e]) + (double)(xb[e] * xb[e]);
-    ss = head_sum(ss, mask);
-    const double inv = 1.0 / sqrt(ss / D + (double)p.eps);
-    double ya[4], yb[4];
-    if (ss > 1e-20 && ss < 1e30) {  // no product below leaves fp32's range
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float ta = xa[e] * wa[e], tb = xb[e] * wb[e];
-        ya[e] = ((double)(ta * r.ca[e]) - (double)(tb * r.sa[e])) * inv;
-        yb[e] = ((double)(tb * r.cb[e]) + (double)(ta * r.sb[e])) * inv;
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const double na = (double)xa[e] * inv * (double)wa[e], nb = (double)xb[e] * inv * (double)wb[e];
-        ya[e] = na * (double)r.ca[e] - nb * (double)r.sa[e];
-        yb[e] = nb * (double)r.cb[e] + na * (double)r.sb[e];
-      }
+    for (int e = 0; e < 4; ++e) {
+      ss = fmaf(xa[e], xa[e], fmaf(xb[e], xb[e], ss));
+      // x w has 16 bits and x w c 24: only the sum rounds
+      const float ta = xa[e] * wa[e], tb = xb[e] * wb[e];
+      da[e] = fmaf(ta, r.ca[e], -(tb * r.sa[e]));
+      db[e] = fmaf(tb, r.cb[e], ta * r.sb[e]);
     }
-    const uint32_t lo = key_codes(ya, mask, s_lo), hi = key_codes(yb, mask, s_hi);
+    ss = head_sum(ss, mask);
+    const float inv = __frsqrt_rn(ss * (1.f / D) + p.eps);
+    bool doubt = !(ss > 1e-20f && ss < 1e30f);
+    uint32_t lo = key_codes(da, inv, mask, s_lo, doubt), hi = key_codes(db, inv, mask, s_hi, doubt);
+    if (__any_sync(mask, doubt)) {  // about one head in 200
+      const uint2* kx = reinterpret_cast<const uint2*>(p.qkv + (int64_t)t * p.row_stride + (int64_t)(p.HQ + pair) * D);
+      const uint2* kw = reinterpret_cast<const uint2*>(p.k_norm);
+      const uint2* kc = reinterpret_cast<const uint2*>(p.cos + (int64_t)t * D);
+      const uint2* ks = reinterpret_cast<const uint2*>(p.sin + (int64_t)t * D);
+      const KeyCodes k = U > 1 ? exact_key_call(kx, kw, kc, ks, p.eps, i, mask) : exact_key(kx, kw, kc, ks, p.eps, i, mask);
+      lo = k.lo;
+      hi = k.hi;
+      s_lo = k.s_lo;
+      s_hi = k.s_hi;
+    }
     store_k(rec + 64 * token, lo, hi, i, mask);
   }
   if ((i & 7) == 0) {  // groups i / 8 (low channels) and 2 + i / 8
@@ -379,7 +417,8 @@ extern "C" int ffb_qk_norm_rope_kv4(const uint16_t* qkv, int64_t row_stride, con
   // with four
   const bool many = T >= 4 * ffb::sm_count();
   const int heads = (many ? 4 : 1) * 2 * WARPS, q_chunks = (HQ + heads - 1) / heads;
-  const dim3 grid(T, q_chunks + (2 * HK + 2 * WARPS - 1) / (2 * WARPS));
+  const int rows = T < 65535 ? T : 65535;
+  const dim3 grid(q_chunks + (2 * HK + 2 * WARPS - 1) / (2 * WARPS), rows, (T + rows - 1) / rows);
   cudaError_t e = many ? ffb::launch(kv4_write_kernel<4>, grid, dim3(WARPS * 32), 0, (cudaStream_t)stream, a, q_chunks)
                        : ffb::launch(kv4_write_kernel<1>, grid, dim3(WARPS * 32), 0, (cudaStream_t)stream, a, q_chunks);
   if (e != cudaSuccess) return ffb::fail(FFB_ECUDA, "%s: %s", who, cudaGetErrorString(e));
