@@ -4,11 +4,16 @@
 //   n = x / sqrt(mean(x^2) + eps) * w,  y[i] = n[i] c[i] - n[i + 64] s[i]   (i < 64)
 //                                       y[i] = n[i] c[i] + n[i - 64] s[i]   (i >= 64)
 // with the queries rounded once to bf16 and the keys and values quantised straight into the
-// cache.  Bound by HBM: a row reads 256 (HQ + 2 HK) + 512 bytes and writes 256 HQ + 144 HK.
+// cache.  A row reads 256 (HQ + 2 HK) + 512 bytes and writes 256 HQ + 144 HK.
 // Sixteen lanes take one (row, head): lane i holds channels 4i..4i+3 and 64+4i.., so the
 // rotation needs no exchange and a scale group is eight lanes.  A CTA takes one row: the first
 // ones of a row its query heads (four to a half warp once there are enough rows, their loads
-// issued together), the last its key and value heads.
+// issued together), the last its key and value heads; a row's CTAs are launched next to each
+// other, so that the quantiser's arithmetic runs beside the queries' traffic (behind it: 78 us
+// where this takes 74.6).
+// Measured: 7128 rows of 64 + 8 heads (275 MB) 70.5 us, 3.9 TB/s, of which the queries alone would
+// take 45; the rest is the codes' instructions.  One row of 32 + 8 heads 3.4 us, 320 rows 6.4 us:
+// launch and latency.  Reading those 7128 rows back 11.0 us, 3.4 TB/s.
 //
 // The codes are those of the formula in exact arithmetic, up to fp64's rounding: a key next to
 // the border of two codes must not fall to either side by chance.  Keys are worked out in fp32 with

@@ -21,6 +21,11 @@ code written against the reference runs unchanged:
     vision_linear / vision_attention: the HF vision blocks' nn.Linear (+ residual / GELU)
                        and SDPA (_legacy/vision_graph_runtime.py:16-27)
 
+Beyond the reference, whose keys and values live within one forward pass: a paged K/V cache held
+in 4 bits.  `kv4_pages` allocates it, `qk_pair_kv4` writes new rows (`qk_pair` whose keys and
+values end in the cache), `attention_kv4` attends over it (single tokens to long chunks, sliding
+window with sinks), `kv4_read` reads rows back.
+
 Outputs are allocated with torch on the input's device (stream-ordered, graph-safe
 through the caching allocator).  Argument errors raise ValueError (the reference uses
 assert); CUDA failures raise FFBError.  There is no CPU path.
@@ -500,8 +505,9 @@ def attention_kv4(q, pages, page_table, row_start, ctx_len, scale, window=0, sin
     returns it (the rows' own keys are in the cache already); page_table, row_start, ctx_len as
     there.  window > 0: a row at position p sees keys p - window + 1 .. p and the first `sinks`.
     A row that sees nothing gets zeros.  max_rows: the most rows of one sequence in this call, if
-    known (it sizes the launch; default T, right for any mix).  Returns [T, HQ, 128] bf16 (`out`,
-    or a new tensor; rows of no sequence are left as they were)."""
+    known (it sizes the launch and changes no result beyond rounding; default T / B, rounded up).
+    Held values must be below 2^57 in size.  Returns [T, HQ, 128] bf16 (`out`, or a new tensor; rows
+    of no sequence are left as they were)."""
     place, where, b = _kv4_place(pages, page_table, row_start, ctx_len)
     dev = pages.device
     if q.dtype is not BF16 or q.device != dev:
@@ -510,7 +516,7 @@ def attention_kv4(q, pages, page_table, row_start, ctx_len, scale, window=0, sin
     (hq, t, _), hk = q.shape, pages.shape[1]
     if hq <= 0 or hq % hk:
         _need(False, f"{hq} query heads for {hk} K/V heads")
-    most = t if max_rows is None else min(max_rows, t)
+    most = -(-t // max(b, 1)) if max_rows is None else min(max_rows, t)
     _need(most > 0 or t == 0, "max_rows must be positive")
     y = _kv4_out(out, q, (t, hq, 128))
     if t:

@@ -472,7 +472,8 @@ int ffb_attention_full(const uint16_t* q, const uint16_t* k, const uint16_t* v, 
  * pages [num_pages][HK][FFB_KV4_RECORD] u8, 16-byte aligned: a page holds 64 tokens, and per
  * K/V head one record of codes and scales (layout: csrc/kv4.cuh).  A group of 32 channels
  * shares a scale s, the smallest number of five significant bits >= max|x| / 7 (bf16); a code
- * is rint(x / s) in -7..7.  Every held value is exact in bf16.
+ * is rint(x / s) in -7..7.  Every held value is exact in bf16.  A group whose largest |x| is below
+ * 2^-100 is held as zeros, one with a value that is not finite or reaches 2^127 as NaN.
  *
  * Every entry takes the same description of its T rows, on the device: row_start [B+1]
  * (ascending): rows [row_start[b], row_start[b+1]) are sequence b's newest tokens (none, one
@@ -508,9 +509,11 @@ int ffb_kv4_read(const uint8_t* pages, int num_pages, const int* page_table, int
  * them: write them first).  q [HQ, T, 128], out [T, HQ*128] bf16, 16-byte aligned.  window > 0:
  * row at position p sees keys j <= p with p - j < window or j < sinks; pages that no row sees
  * are not read.  window 0: every key j <= p (sinks must be 0).  A row that sees no key gets
- * zeros.  max_rows: the most rows that a sequence has in this call (1..T); it sizes the grid,
- * longer sequences are still computed, only slower.  ws: ffb_attention_kv4_workspace(...)
- * bytes, 16-byte aligned (NULL when 0), scratch of this call alone. */
+ * zeros; one that sees a NaN key becomes NaN, one that sees a NaN value is NaN in that group of
+ * channels at least.  Held values must be below 2^57 in size.  max_rows: the most rows that a
+ * sequence has in this call (1..T); it sizes the grid, longer sequences are still computed, only
+ * slower.  ws: ffb_attention_kv4_workspace(...) bytes, 16-byte aligned (NULL when 0), scratch of
+ * this call alone. */
 int ffb_attention_kv4(const uint16_t* q, const uint8_t* pages, int num_pages, const int* page_table,
                       int64_t table_stride, int max_pages, const int* row_start, const int* ctx_len,
                       uint16_t* out, void* ws, int64_t ws_bytes, int B, int T, int max_rows, int HQ, int HK,

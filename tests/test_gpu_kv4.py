@@ -153,7 +153,7 @@ def test_decode(hq, hk, ctx):
 
 
 @pytest.mark.parametrize("rows,ctx", [([2], [2]), ([5, 1, 0, 3], [70, 1, 40, 64]), ([17], [200]), ([64, 33], [64, 500]),
-                                      ([130], [1200]), ([200, 1], [263, 900])])
+                                      ([130], [1200]), ([200, 1], [263, 900]), ([8, 6, 1], [300, 77, 1]), ([9, 11], [9, 130])])
 @pytest.mark.parametrize("hq,hk", [(4, 1), (4, 4), (16, 2), (3, 1)])
 def test_chunks(rows, ctx, hq, hk):
     _attend(rows, ctx, hq, hk, seed=len(rows) + hq, max_rows=max(rows), tail=1)
@@ -171,11 +171,20 @@ def test_max_rows_is_only_a_hint(max_rows):
 
 
 @pytest.mark.parametrize("rows,ctx", [([300, 0, 7, 129], [500, 3, 7, 64]), ([65], [700]), ([64], [64]), ([513, 1], [515, 1300])])
-def test_long_chunks_with_a_small_hint(rows, ctx):
+@pytest.mark.parametrize("hint", [5, 8, 9, 64])
+def test_long_chunks_with_a_small_hint(rows, ctx, hint):
     """More query tiles than the launch was sized for: a CTA takes several, one or both halves
     of the last, tiles of no key among them."""
-    _attend(rows, ctx, 8, 2, seed=31, max_rows=5, lead=3, tail=2)
-    _attend(rows, ctx, 8, 2, seed=32, max_rows=5, window=70, sinks=5)
+    _attend(rows, ctx, 8, 2, seed=31, max_rows=hint, lead=3, tail=2)
+    _attend(rows, ctx, 8, 2, seed=32, max_rows=hint, window=70, sinks=5)
+
+
+def test_more_items_than_processors():
+    """Long chunks of many sequences: whole items first, the last wave's cut, some sequences without
+    rows or keys."""
+    rows, ctx = [64, 70, 0, 64, 1, 130, 64], [640, 70, 40, 300, 0, 1000, 64]
+    _attend(rows, ctx, 96, 24, seed=5, max_rows=130, lead=2, tail=3)
+    _attend(rows, ctx, 96, 24, seed=6, max_rows=40, window=90, sinks=2)
 
 
 @pytest.mark.parametrize("seed", range(4))
@@ -200,6 +209,7 @@ def test_rows_that_see_nothing_are_zero():
 def test_scales(scale):
     """scale 30 gives scores of thousands: the running maximum has to carry them."""
     _attend([1, 6], [333, 70], 8, 2, seed=4, scale=scale, max_rows=6)
+    _attend([1, 20], [333, 70], 8, 2, seed=7, scale=scale, max_rows=20)
     _attend([1, 1, 1], [333, 70, 1], 8, 2, seed=5, scale=scale, max_rows=1)
     _attend([1, 2], [900, 2], 16, 2, seed=6, scale=scale, max_rows=2, window=100, sinks=1)
 
