@@ -33,7 +33,7 @@
 // the shares and their join.  Tried and slower: blocks of 64 keys with S held twice (653 us: an MMA
 // of N 64 costs as much as one of 128), four warps for K and four for V (631), a fourth slot for three
 // raw pages (618), a row's scores kept in registers beside four dequantising warps (668), some of
-// the exponentials on the multiply-add pipe (no gain at an eighth, 4% slower at a quarter).
+// the exponentials on the multiply-add pipe (an eighth no gain, a quarter 4% slower).
 #include "kv4.cuh"
 #include "pdl.cuh"
 
