@@ -20,6 +20,14 @@ def quantize(x):
     return codes.reshape(x.shape), scale
 
 
+def held(x):
+    """What the cache holds of any x [..., 128] fp64: groups below 2^-100 as zeros, groups with a value
+    that is not finite or reaches 2^127 as NaN."""
+    top = x.abs().reshape(*x.shape[:-1], 4, 32).amax(-1).repeat_interleave(32, -1)  # a NaN stays one
+    bad = ~(top < 2.0 ** 127)
+    return values(*quantize(x.masked_fill(bad | (top < 2.0 ** -100), 0.0))).masked_fill(bad, float("nan"))
+
+
 def values(codes, scale):
     return codes * scale.repeat_interleave(32, -1)
 

@@ -1,6 +1,9 @@
 """The 4-bit K/V cache on the GPU: its writer, its reader and the attention over it, against
 plain formulas in 64 bits (tests/_kv4.py)."""
+import subprocess
+import sys
 import types
+from pathlib import Path
 
 import pytest
 import torch
@@ -12,6 +15,7 @@ from tests import _kv4 as ref
 pytestmark = pytest.mark.gpu
 BF16 = torch.bfloat16
 DEV = "cuda"
+
 
 @pytest.fixture(autouse=True)
 def _no_device_error():
@@ -47,7 +51,7 @@ def _dev(x):
     return x.to(DEV)
 
 
-def _written(rows, ctx, hq, hk, seed, lead=0, tail=0, edit=None):
+def _written(rows, ctx, hq, hk, seed, lead=0, tail=0, edit=None, weight=None):
     """Runs the writer on random rows; returns everything host-side."""
     table, starts, lens, num = _batch(rows, ctx, hk, seed, lead=lead)
     total = int(starts[-1]) + tail
@@ -58,6 +62,8 @@ def _written(rows, ctx, hq, hk, seed, lead=0, tail=0, edit=None):
     angle = torch.rand(total, 128, generator=g) * 6.3
     cos, sin = angle.cos().to(BF16), angle.sin().to(BF16)  # 128 independent columns
     qn, kn = _norm(seed + 2), _norm(seed + 3)
+    if weight is not None:
+        kn.weight = weight
     pages = ops.kv4_pages(num, hk)
     out = torch.full((hq, total, 128), 7.0, dtype=BF16, device=DEV)
     yq = ops.qk_pair_kv4(_dev(qkv), _dev(qn), _dev(kn), _dev(cos), _dev(sin), pages, _dev(table), _dev(starts),
@@ -68,7 +74,8 @@ def _written(rows, ctx, hq, hk, seed, lead=0, tail=0, edit=None):
 
 @pytest.mark.parametrize("rows,ctx,hq,hk", [
     ([1], [1], 4, 2), ([1], [64], 8, 8), ([1], [65], 5, 1), ([3, 0, 70], [3, 9, 200], 8, 2), ([130], [131], 16, 4),
-    ([1] * 9, [1, 2, 63, 64, 65, 127, 128, 129, 1000], 32, 8)])
+    ([1] * 9, [1, 2, 63, 64, 65, 127, 128, 129, 1000], 32, 8), ([600, 0, 113], [611, 5, 500], 6, 3),
+    ([700], [700], 5, 1)])
 def test_write_and_read_back(rows, ctx, hq, hk):
     c = _written(rows, ctx, hq, hk, seed=11 + len(rows), lead=2, tail=3)
     q, k, v = ref.norm_rotate_quantize(c.qkv, c.qn, c.kn, c.cos, c.sin, hq, hk)
@@ -109,6 +116,27 @@ def test_write_of_special_values():
     assert (gv[0, 3, :32] == 0).all()
     assert gv[0, 4, :32].isnan().all()
     assert gv[0, 5, :4].tolist() == [7.0, -4.0, 0.0, 2.0]  # ties to the even code
+
+
+@pytest.mark.parametrize("rows", [40, 640])
+def test_keys_of_any_size(rows):
+    """Rows and norm weights from tiny to huge, rows of zeros: where fp32 leaves its range the keys are
+    still the formula's."""
+    def edit(x):
+        x.mul_(torch.logspace(-30, 25, rows)[:, None])
+        x[3] = 0
+        x[5, ::3] *= 2.0 ** -40
+
+    weight = _norm(9).weight.float()
+    weight[0:40] *= 1e-28
+    weight[70:90] *= 1e20
+    weight[100:128] *= 1e34
+    c = _written([rows], [rows + 3], 4, 1, seed=41, edit=edit, weight=weight.to(BF16))
+    x = c.qkv.double().reshape(rows, -1, 128).transpose(0, 1)
+    k, v = ref.held(ref.norm_rotate(x[4:5], c.kn, c.cos, c.sin)), ref.held(x[5:])
+    gk, gv = (x.cpu().double() for x in ops.kv4_read(c.pages, _dev(c.table), _dev(c.starts), _dev(c.lens), rows))
+    assert torch.equal(gk.isnan(), k.isnan()) and torch.equal(gk.nan_to_num(0), k.nan_to_num(0))
+    assert torch.equal(gv.isnan(), v.isnan()) and torch.equal(gv.nan_to_num(0), v.nan_to_num(0))
 
 
 def test_write_strided_rows_and_single_row():
@@ -364,23 +392,79 @@ def test_decoding_steps_in_a_captured_graph():
         assert ((out.cpu().double() - want).abs() <= limit).all()
 
 
-def test_another_stream_and_two_calls_at_once():
-    rows, ctx, hq, hk = [1, 1], [3000, 700], 8, 2
-    table, starts, lens, num = _batch(rows, ctx, hk, 13)
-    g = torch.Generator().manual_seed(3)
+def _long_cache(rows, hq, hk, seed):
+    table, starts, lens, num = _batch([rows, rows], [3000, 700], hk, seed)
+    g = torch.Generator().manual_seed(seed)
     pages = _dev(ref.pack(*(torch.randn(num, hk, 64, 128, generator=g, dtype=torch.float64) for _ in range(2))))
-    q = torch.randn(hq, 2, 128, generator=g).to(BF16).to(DEV)
-    place = (pages, _dev(table), _dev(starts), _dev(lens))
-    first = ops.attention_kv4(q, *place, 0.1, max_rows=1)
+    q = torch.randn(hq, 2 * rows, 128, generator=g).to(BF16).to(DEV)
+    return q, (pages, _dev(table), _dev(starts), _dev(lens))
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_another_stream_and_two_calls_at_once(rows):
+    q, place = _long_cache(rows, 8, 2, 13)
+    first = ops.attention_kv4(q, *place, 0.1, max_rows=rows)
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in range(2)]
     outs = []
     for s in streams:
         with torch.cuda.stream(s):
             for _ in range(5):
-                outs.append(ops.attention_kv4(q, *place, 0.1, max_rows=1))
+                outs.append(ops.attention_kv4(q, *place, 0.1, max_rows=rows))
     torch.cuda.synchronize()
     assert all(torch.equal(o, first) for o in outs)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_captured_calls_with_workspaces(rows):
+    """Shares of long sequences joined in a replayed graph, the lengths changed between replays, two
+    graphs at once on two streams."""
+    q, place = _long_cache(rows, 8, 2, 14)
+    lens = place[3]
+    ops.attention_kv4(q, *place, 0.1, max_rows=rows)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(ops.attention_kv4(q, *place, 0.1, max_rows=rows))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for grow in (0, -37, 20, -400):
+        lens.add_(grow)
+        want = ops.attention_kv4(q, *place, 0.1, max_rows=rows)
+        for o in outs:
+            o.fill_(7)
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for graph, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want) for o in outs)
+
+
+@pytest.mark.parametrize("rows", [1, 100])
+def test_first_call_of_a_process_is_captured(rows):
+    """Nothing that a call sets up once (attributes, symbols, modules) disturbs a capture."""
+    code = f"""
+import torch
+from fastforward_b200 import ops
+pages = ops.kv4_pages(8, 2)
+table = torch.arange(8, dtype=torch.int32, device="cuda")[None]
+starts = torch.tensor([0, {rows}], dtype=torch.int32, device="cuda")
+lens = torch.tensor([300], dtype=torch.int32, device="cuda")
+q = torch.randn(8, {rows}, 128, device="cuda").bfloat16()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = ops.attention_kv4(q, pages, table, starts, lens, 0.1)
+    k, v = ops.kv4_read(pages, table, starts, lens, {rows})
+graph.replay()
+torch.cuda.synchronize()
+assert (y == 0).all() and (k == 0).all() and (v == 0).all()
+"""
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=300, cwd=Path(__file__).resolve().parents[1])
 
 
 def test_pages_past_32_bits():
