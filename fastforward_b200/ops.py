@@ -415,31 +415,34 @@ def kv4_pages(num_pages, heads, device="cuda"):
 
 
 def _kv4_place(pages, page_table, row_start, ctx_len):
-    """Checks the cache and the rows' description; returns the C entries' common arguments."""
-    dev = pages.device
-    if not (pages.is_cuda and page_table.device == row_start.device == ctx_len.device == dev):
+    """Checks the cache and the rows' description; returns the C entries' common arguments, the device's
+    index, the sequences and the K/V heads."""
+    dev = pages.get_device()  # -1: CPU
+    if dev < 0 or not (page_table.get_device() == row_start.get_device() == ctx_len.get_device() == dev):
         _need(False, "CUDA tensors of one device required (no CPU fallback)")
-    if not (pages.dtype is torch.uint8 and pages.dim() == 3 and pages.shape[2] == L.KV4_RECORD and pages.is_contiguous()):
+    shape, table = pages.shape, page_table.shape
+    if not (pages.dtype is torch.uint8 and len(shape) == 3 and shape[2] == L.KV4_RECORD and pages.is_contiguous()):
         _need(False, f"pages must be contiguous uint8 [pages, heads, {L.KV4_RECORD}]")
     if not (page_table.dtype is row_start.dtype is ctx_len.dtype is torch.int32):
         _need(False, "page_table, row_start and ctx_len must be int32")
-    if page_table.dim() != 2 or (page_table.stride(1) != 1 and page_table.shape[1] != 1):
+    stride = page_table.stride()
+    if len(table) != 2 or (stride[1] != 1 and table[1] != 1):
         _need(False, "page_table [B, width], unit last stride")
-    b, width = page_table.shape
+    b, width = table
     if not (row_start.shape == (b + 1,) and ctx_len.shape == (b,) and row_start.is_contiguous() and ctx_len.is_contiguous()):
         _need(False, f"row_start [{b + 1}] and ctx_len [{b}], contiguous")
-    return (pages.data_ptr(), pages.shape[0], page_table.data_ptr(), page_table.stride(0), width), (
-        row_start.data_ptr(), ctx_len.data_ptr()), b
+    return (pages.data_ptr(), shape[0], page_table.data_ptr(), stride[0], width, row_start.data_ptr(),
+            ctx_len.data_ptr()), dev, b, shape[1]
 
 
-def _kv4_call(device, name, *args):
-    """`call` on `device`'s current stream, with that device current."""
+def _kv4_call(dev, name, *args):
+    """`call` on the current stream of device number `dev`, with that device current."""
     fn = getattr(L.lib(), name)
-    if torch._C._cuda_getDevice() == device.index:
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    if torch._C._cuda_getDevice() == dev:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     if rc:
         L.check(rc)
 
@@ -467,36 +470,40 @@ def qk_pair_kv4(qkv, qn, kn, cos, sin, pages, page_table, row_start, ctx_len, ou
     b, whose cache holds ctx_len[b] tokens with them, in the pages of page_table[b].  Returns
     the queries [HQ, T, 128] (`out`, or a new tensor; rows of no sequence are left as they
     were).  Norm, rotation and quantisation run in one pass; the queries round once to bf16."""
-    place, rows, b = _kv4_place(pages, page_table, row_start, ctx_len)
-    qw, kw, eps, dev = qn.weight, kn.weight, qn.variance_epsilon, pages.device
+    place, dev, b, hk = _kv4_place(pages, page_table, row_start, ctx_len)
+    qw, kw, eps = qn.weight, kn.weight, qn.variance_epsilon
     if not (qkv.dtype is qw.dtype is kw.dtype is cos.dtype is sin.dtype is BF16):
         _need(False, "bf16 required")
-    if not (qkv.device == qw.device == kw.device == cos.device == sin.device == dev):
+    if not (qkv.get_device() == qw.get_device() == kw.get_device() == cos.get_device() == sin.get_device() == dev):
         _need(False, "tensors on one device")
-    _need(qkv.dim() == 2 and qkv.stride(1) == 1, "qkv [T, (HQ + 2 HK) * 128], unit last stride")
-    (t, width), hk = qkv.shape, pages.shape[1]
+    shape, stride = qkv.shape, qkv.stride()
+    if len(shape) != 2 or stride[1] != 1:
+        _need(False, "qkv [T, (HQ + 2 HK) * 128], unit last stride")
+    t, width = shape
     hq = width // 128 - 2 * hk
     if width % 128 or hq <= 0 or hq % hk:
         _need(False, f"qkv width {width} does not fit {hk} K/V heads")
-    _need(abs(eps - kn.variance_epsilon) < 1e-12, "q_norm and k_norm must share eps")
-    _need(qw.shape == kw.shape == (128,) and qw.is_contiguous() and kw.is_contiguous(), "norm weights [128]")
-    _need(cos.numel() == sin.numel() == t * 128 and cos.shape[-1] == sin.shape[-1] == 128, "cos, sin [T, 128]")
+    if not abs(eps - kn.variance_epsilon) < 1e-12:
+        _need(False, "q_norm and k_norm must share eps")
+    if not (qw.shape == kw.shape == (128,) and qw.is_contiguous() and kw.is_contiguous()):
+        _need(False, "norm weights [128]")
+    if not (cos.numel() == sin.numel() == t * 128 and cos.shape[-1] == sin.shape[-1] == 128):
+        _need(False, "cos, sin [T, 128]")
     cos, sin = cos.contiguous(), sin.contiguous()  # held until the launch is enqueued
     yq = _kv4_out(out, qkv, (hq, t, 128))
     if t:
-        _kv4_call(dev, "ffb_qk_norm_rope_kv4", qkv.data_ptr(), qkv.stride(0) if t > 1 else width, qw.data_ptr(),
-                  kw.data_ptr(), eps, cos.data_ptr(), sin.data_ptr(), yq.data_ptr(), *place, *rows, b, t, hq, hk)
+        _kv4_call(dev, "ffb_qk_norm_rope_kv4", qkv.data_ptr(), stride[0] if t > 1 else width, qw.data_ptr(),
+                  kw.data_ptr(), eps, cos.data_ptr(), sin.data_ptr(), yq.data_ptr(), *place, b, t, hq, hk)
     return yq
 
 
 def kv4_read(pages, page_table, row_start, ctx_len, rows):
     """The newest rows as the 4-bit cache holds them: k, v [HK, rows, 128] bf16, exact.  To read
     whole sequences, pass row_start with ctx_len's running sums."""
-    place, where, b = _kv4_place(pages, page_table, row_start, ctx_len)
-    hk = pages.shape[1]
-    k, v = torch.empty((2, hk, rows, 128), device=pages.device, dtype=BF16).unbind(0)
+    place, dev, b, hk = _kv4_place(pages, page_table, row_start, ctx_len)
+    k, v = (pages.new_empty((hk, rows, 128), dtype=BF16) for _ in range(2))
     if rows:
-        _kv4_call(pages.device, "ffb_kv4_read", *place, *where, k.data_ptr(), v.data_ptr(), b, rows, hk)
+        _kv4_call(dev, "ffb_kv4_read", *place, k.data_ptr(), v.data_ptr(), b, rows, hk)
     return k, v
 
 
@@ -508,20 +515,22 @@ def attention_kv4(q, pages, page_table, row_start, ctx_len, scale, window=0, sin
     known (it sizes the launch and changes no result beyond rounding; default T / B, rounded up).
     Held values must be below 2^57 in size.  Returns [T, HQ, 128] bf16 (`out`, or a new tensor; rows
     of no sequence are left as they were)."""
-    place, where, b = _kv4_place(pages, page_table, row_start, ctx_len)
-    dev = pages.device
-    if q.dtype is not BF16 or q.device != dev:
+    place, dev, b, hk = _kv4_place(pages, page_table, row_start, ctx_len)
+    if q.dtype is not BF16 or q.get_device() != dev:
         _need(False, "q must be bf16, on the cache's device")
-    _need(q.dim() == 3 and q.shape[2] == 128 and q.is_contiguous(), "q must be contiguous [HQ, T, 128]")
-    (hq, t, _), hk = q.shape, pages.shape[1]
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != 128 or not q.is_contiguous():
+        _need(False, "q must be contiguous [HQ, T, 128]")
+    hq, t, _ = shape
     if hq <= 0 or hq % hk:
         _need(False, f"{hq} query heads for {hk} K/V heads")
     most = -(-t // max(b, 1)) if max_rows is None else min(max_rows, t)
-    _need(most > 0 or t == 0, "max_rows must be positive")
+    if most <= 0 and t:
+        _need(False, "max_rows must be positive")
     y = _kv4_out(out, q, (t, hq, 128))
     if t:
-        need = _kv4_workspace(dev.index, b, t, hq, hk, most, place[4], window, sinks)
+        need = _kv4_workspace(dev, b, t, hq, hk, most, place[4], window, sinks)
         ws = pages.new_empty(need) if need else None
-        _kv4_call(dev, "ffb_attention_kv4", q.data_ptr(), *place, *where, y.data_ptr(), ws.data_ptr() if need else None,
+        _kv4_call(dev, "ffb_attention_kv4", q.data_ptr(), *place, y.data_ptr(), ws.data_ptr() if need else None,
                   need, b, t, most, hq, hk, scale, window, sinks)
     return y
