@@ -12,7 +12,8 @@
 //     STAGES such halves, filled by cp.async.bulk: no warp waits for another inside a share, and
 //     page ids are read 32 at a time, so no load waits for one;
 //   - the CTAs share out the pages of all items in equal runs, whatever the lengths of the
-//     sequences (they are on the device, so every CTA sums them up itself); an item cut by a run's
+//     sequences (they are on the device, so every CTA sums them up itself), or, where these are even
+//     enough, take an item each; an item cut by a run's
 //     end leaves fp32 partials, which the CTA that has its last page adds up at the end of its own
 //     run (it waits only for CTAs before it; a second launch cost 6 us).  With few pages an item
 //     (WHOLE) each item is one CTA's.  The first pages and the queries of a CTA's next item are on
@@ -73,6 +74,10 @@ constexpr float UNSEEN = 3e38f;       // 64 - maximum before the first score: fi
 
 constexpr int MIN_PAGES = GROUPS;     // fewest pages worth a CTA: one a group
 constexpr int ITEM_PAGES = 8;         // what starting and ending an item takes, in pages
+// Items are not cut where the longest has at most so many pages more than an equal run: us apart / cut,
+// 32 + 8 heads, 32 sequences of 256 tokens 10.6 / 17.6, of 2048 tokens 28.1 / 33.6 (5 pages more); 8 of
+// 640 tokens (14 more) 15.0 / 13.3.
+constexpr int APART = 10;
 
 // Sequence b's rows, pages and items in the run of pages that the CTAs share: its items, HK for
 // each tile of `qt` columns, one after the other, each with ITEM_PAGES for its start and end and
@@ -120,7 +125,7 @@ struct Shape {
   static constexpr int STAGES = NT == 1 ? 2 : 4;  // half pages in a warp's ring
   static constexpr int RING = WARPS * STAGES * HALF_BYTES;
   static constexpr int EXCHANGE = WARPS * (2 * 8 * NT + 8 * CS) * 4;
-  static constexpr int BARS = WARPS * STAGES * 8 + WARPS * 8 + sizeof(Run) + 16;
+  static constexpr int BARS = WARPS * STAGES * 8 + WARPS * 16 + sizeof(Run) + 16;
   // ring | exchange | Q fragments [NT][4][32] uint4 | query rows [8 NT][QROW], of this and the next item |
   // sums of 8 q [8 NT][4] | column factors, positions | barriers, schedule
   static constexpr int SMEM = RING + EXCHANGE + NT * 4 * 512 + 2 * 8 * NT * QROW + NT * 128 + NT * 64 + BARS + 128;
@@ -256,7 +261,8 @@ __global__ void __launch_bounds__(THREADS, Shape<NT>::PER_SM) kv4_attention_kern
   int* spos = reinterpret_cast<int*>(smul + 8 * NT);                                   // [8 NT]
   uint64_t* full = reinterpret_cast<uint64_t*>(spos + 8 * NT);
   int64_t* sums = reinterpret_cast<int64_t*>(full + WARPS * STAGES);  // [WARPS]
-  Run& run = *reinterpret_cast<Run*>(sums + WARPS);
+  int2* spans = reinterpret_cast<int2*>(sums + WARPS);                // [WARPS]
+  Run& run = *reinterpret_cast<Run*>(spans + WARPS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(&run + 1);
 
   const Seqs& sv = args.seqs;
@@ -284,27 +290,67 @@ __global__ void __launch_bounds__(THREADS, Shape<NT>::PER_SM) kv4_attention_kern
   } else {
     const int per = (sv.B + THREADS - 1) / THREADS, b_lo = min(tid * per, sv.B), b_hi = min(b_lo + per, sv.B);
     int64_t mine = 0;
-    for (int i = b_lo; i < b_hi; ++i) mine += seq_at(args, i, QT).weight(sv.HK);
+    int longest = 0, count = 0;
+    for (int i = b_lo; i < b_hi; ++i) {
+      const Seq q = seq_at(args, i, QT);
+      mine += q.weight(sv.HK);
+      count += q.tiles * sv.HK;
+      if (q.tiles > 0) longest = max(longest, ITEM_PAGES + q.pages());
+    }
     int64_t scan = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const int64_t v = __shfl_up_sync(0xffffffffu, scan, d);
       if (lane >= d) scan += v;
     }
-    if (lane == 31) sums[warp] = scan;
+    const int2 span = make_int2(__reduce_max_sync(0xffffffffu, longest), __reduce_add_sync(0xffffffffu, count));
+    if (lane == 31) {
+      sums[warp] = scan;
+      spans[warp] = span;
+    }
     __syncthreads();
     int64_t pre = scan - mine;
+    int items = 0;
     total = 0;
     for (int w = 0; w < WARPS; ++w) {
       if (w < warp) pre += sums[w];
       total += sums[w];
+      longest = max(longest, spans[w].x);
+      items += spans[w].y;
     }
     sharing = (int)max((int64_t)1, min((int64_t)gridDim.x, total / MIN_PAGES));
     if ((int)blockIdx.x >= sharing) return;
     at = mul_div(blockIdx.x, total, sharing);
-    const int64_t end = mul_div(blockIdx.x + 1, total, sharing);
-    if (at >= end) return;  // no rows at all
-    if (at >= pre && at < pre + mine) {
+    int64_t end = mul_div(blockIdx.x + 1, total, sharing);
+    if (items <= sharing && longest <= APART + end - at) {  // an item each, none cut
+      if ((int)blockIdx.x >= items) return;
+      int before = count;
+      for (int d = 1; d < 32; d <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, before, d);
+        if (lane >= d) before += v;
+      }
+      before -= count;
+      for (int w = 0; w < warp; ++w) before += spans[w].y;
+      int k = (int)blockIdx.x - before;
+      if (k >= 0 && k < count) {
+        for (int i = b_lo;; ++i) {
+          const Seq seq = seq_at(args, i, QT);
+          const int n = seq.tiles * sv.HK;
+          if (k < n) {
+            run.left = ITEM_PAGES + seq.pages();
+            run.b = i;
+            run.item = k;
+            run.from = -ITEM_PAGES;
+            break;
+          }
+          k -= n;
+        }
+      }
+      end = at;  // found
+    } else if (at >= end) {
+      return;  // no rows at all
+    }
+    if (at < end && at >= pre && at < pre + mine) {
       int i = b_lo;
       int64_t p = pre;
       for (;; ++i) {
@@ -904,7 +950,8 @@ __global__ void __launch_bounds__(256) kv4_join_tc_kernel(const AttnArgs args) {
 
 // How a call is laid out.  kernel: 1 / 2 = the register path with 8 / 16 query columns a CTA,
 // TC = the tensor-memory path with 256.  splits: the shares of the pages of each of TC's first
-// `cut` items, behind which come `whole` items of one CTA; the register path has 1 (every item one CTA's) or 0 (all pages in equal runs).
+// `cut` items, behind which come `whole` items of one CTA; the register path has 1 (every item one
+// CTA's) or 0 (all pages in equal runs).
 constexpr int TC = 3;
 struct Plan {
   int kernel, tiles, splits, ctas, cut, whole;
@@ -964,8 +1011,10 @@ Plan make_plan(int B, int T, int HQ, int HK, int max_rows, int max_pages, int wi
     const int64_t all = (int64_t)T * (HQ / HK) / 256 + B;
     plan_tc(p, (int64_t)HK * (all < B * tiles ? all : B * tiles), pages, sms);
   } else {
-    // an item of up to two pages a warp group is done sooner than a second launch
-    p.splits = pages <= 2 * GROUPS ? 1 : 0;
+    // Narrow tables: each item one CTA's, without a look at all lengths.  us so / in runs, 32 + 8 heads: one
+    // sequence of 1024 tokens 11.6 / 12.3, of 1536 14.5 / 13.0; 8 of 1536 15.1 / 16.4, of 2048 17.8 / 17.8;
+    // 128 of 2048 86 / 93; 32 of 300 to 2048 in one call 23.9 / 24.6.
+    p.splits = pages <= (B * HK * tiles >= 64 ? 32 : 16) ? 1 : 0;
     p.cut = p.whole = 0;
     p.ctas = p.splits ? B * HK : sms * (p.kernel == 1 ? Shape<1>::PER_SM : Shape<2>::PER_SM);
     p.bytes = p.splits ? 0 : (int64_t)p.ctas * 2 * (8 + width * (D + 2) * 4);

@@ -227,6 +227,18 @@ def test_ragged_batches_share_the_pages(seed):
     _attend(rows, ctx, [8, 8, 2, 24][seed], [2, 1, 1, 2][seed], seed=seed, max_rows=2, lead=1, tail=1)
 
 
+@pytest.mark.parametrize("b,hk", [(70, 2), (33, 1), (3, 4), (300, 1)])
+def test_even_lengths_in_a_wide_table(b, hk):
+    """Sequences alike enough that each item is one CTA's, in a table far wider than they need; some
+    have no rows, one no keys."""
+    g = torch.Generator().manual_seed(b)
+    ctx = [int(x) for x in torch.randint(230, 330, (b,), generator=g)]
+    rows = [int(x > 0) for x in torch.randint(0, 8, (b,), generator=g)]
+    rows[1], ctx[1] = 1, 0
+    _attend(rows, ctx, 4 * hk, hk, seed=b, max_rows=1, width=60, lead=1, tail=1)
+    _attend(rows, ctx, 12 * hk, hk, seed=b + 1, max_rows=1, width=60, window=100, sinks=3)
+
+
 def test_rows_that_see_nothing_are_zero():
     """More rows than the sequence holds: the first of them lie before its start."""
     got = _attend([4, 2], [1, 0], 4, 2, seed=2, max_rows=4)
