@@ -513,6 +513,8 @@ def attention_kv4(q, pages, page_table, row_start, ctx_len, scale, window=0, sin
     there.  window > 0: a row at position p sees keys p - window + 1 .. p and the first `sinks`.
     A row that sees nothing gets zeros.  max_rows: the most rows of one sequence in this call, if
     known (it sizes the launch and changes no result beyond rounding; default T / B, rounded up).
+    Single tokens and long chunks are faster in two calls over the same q and out, each with its
+    slice of row_start, ctx_len and page_table.
     Held values must be below 2^57 in size.  Returns [T, HQ, 128] bf16 (`out`, or a new tensor; rows
     of no sequence are left as they were)."""
     place, dev, b, hk = _kv4_place(pages, page_table, row_start, ctx_len)
