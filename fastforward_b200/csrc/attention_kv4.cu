@@ -322,7 +322,8 @@ __global__ void __launch_bounds__(THREADS, Shape<NT>::PER_SM) kv4_attention_kern
     if ((int)blockIdx.x >= sharing) return;
     at = mul_div(blockIdx.x, total, sharing);
     int64_t end = mul_div(blockIdx.x + 1, total, sharing);
-    if (items <= sharing && longest <= APART + end - at) {  // an item each, none cut
+    // one verdict of all CTAs: end - at is not the same in each
+    if (items <= sharing && longest <= APART + mul_div(1, total, sharing)) {  // an item each, none cut
       if ((int)blockIdx.x >= items) return;
       int before = count;
       for (int d = 1; d < 32; d <<= 1) {

@@ -164,9 +164,11 @@ def attention(q, pages, table, starts, lens, scale, window, sinks):
         afterwards: the fp32 steps (two MMAs of 16 products and the subtraction, at most 2^-23 of
         the largest partial sum each, 2^-21 in all) move a score by at most
         2^-21 23 sum_group s_group sum|q|, a probability by that times |scale|, o by twice that;
-      - V's codes may be multiplied with the offset too, sixteen keys at a time: the two MMAs leave
-        at most 2^-23 of 15 sum(p s) and of 8 sum(p s) over those keys (s: the scale of the value's
-        group), 2^-22 23 sum(p s) over all keys, also where every code is 0 and o with it;
+      - V's codes may be multiplied with the offset too, sixteen keys at a time: two MMAs each add
+        sixteen products to the sum, the second taking 8 p s off again.  An adder that lines its 17
+        terms up with the largest and cuts each at 2^-23 of that is off by 17 2^-23 of the largest
+        term, at most 15 sum(p s) over those keys (s: the scale of the value's group): 2^-22 255
+        sum(p s) over all keys, also where every code is 0 and o with it;
       - the result is rounded to bf16: 2^-8 of itself."""
     hq, total, _ = q.shape
     hk = pages.shape[1]
@@ -193,7 +195,7 @@ def attention(q, pages, table, starts, lens, scale, window, sinks):
         mass = (q[:, r0:r1].double().abs().reshape(hq, -1, 4, 32).sum(-1) * top[:, None]).sum(-1).T[..., None]
         sv = pages[table[b, :-(-n // 64)].long()][..., 8704:].contiguous().view(torch.bfloat16).double()
         sv = sv.reshape(-1, hk, 64, 4).transpose(0, 1).reshape(hk, -1, 4)[:, :n].repeat_interleave(hq // hk, 0)
-        limit[r0:r1] += 2.0 ** -22 * 23 * (p @ sv).transpose(0, 1).repeat_interleave(32, -1)
+        limit[r0:r1] += 2.0 ** -22 * 255 * (p @ sv).transpose(0, 1).repeat_interleave(32, -1)
         shift = 2 * abs(scale) * 2.0 ** -21 * 23 * mass
         limit[r0:r1] += spread * (2.0 ** -8 + 2.0 ** -15) * 1.01 + (spread + out[r0:r1].abs()) * shift + out[r0:r1].abs() * 2.0 ** -8 * 1.01
     return out, limit

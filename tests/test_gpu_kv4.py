@@ -239,6 +239,25 @@ def test_even_lengths_in_a_wide_table(b, hk):
     _attend(rows, ctx, 12 * hk, hk, seed=b + 1, max_rows=1, width=60, window=100, sinks=3)
 
 
+@pytest.mark.parametrize("rows,ctx,hq,hk,hint,scale", [
+    ([3, 0, 2, 7, 2, 1, 7, 3, 6, 6, 8, 6, 7, 0, 1, 3, 8, 4, 7, 2],
+     [278, 28, 93, 12, 387, 27, 7, 21, 6, 81, 48, 22, 123, 6, 28, 15, 19, 326, 31, 108], 8, 8, 2, -0.1),
+    ([4, 5, 6, 0, 7, 6, 5, 7, 0, 2, 5, 6, 4, 4, 0, 0, 4, 1, 2, 1],
+     [4, 5, 12, 14, 30, 15, 31, 17, 13, 5, 312, 126, 72, 29, 31, 2, 190, 415, 183, 9], 4, 1, 2, 0.3)])
+def test_short_ragged_sequences_in_a_wide_table(rows, ctx, hq, hk, hint, scale):
+    _attend(rows, ctx, hq, hk, seed=21447, max_rows=hint, width=47, scale=scale, tail=2)
+
+
+@pytest.mark.parametrize("longest", range(520, 1000, 64))
+def test_lengths_at_the_border_of_two_schedules(longest):
+    """One sequence longer than the rest by every number of pages around the one where items begin to
+    be cut: all CTAs take the same side."""
+    rows = [1] * 20
+    for other in (64, 130, 200, 260):
+        _attend(rows, [longest] + [other] * 19, 8, 8, seed=longest + other, max_rows=1, width=47)
+        _attend(rows[:11], [other] * 5 + [longest] + [other + 64] * 5, 4, 1, seed=longest + other, max_rows=1, width=47)
+
+
 def test_rows_that_see_nothing_are_zero():
     """More rows than the sequence holds: the first of them lie before its start."""
     got = _attend([4, 2], [1, 0], 4, 2, seed=2, max_rows=4)
@@ -252,6 +271,13 @@ def test_scales(scale):
     _attend([1, 20], [333, 70], 8, 2, seed=7, scale=scale, max_rows=20)
     _attend([1, 1, 1], [333, 70, 1], 8, 2, seed=5, scale=scale, max_rows=1)
     _attend([1, 2], [900, 2], 16, 2, seed=6, scale=scale, max_rows=2, window=100, sinks=1)
+
+
+def test_a_key_that_holds_nearly_all_weight():
+    """Large scores: one key's value is most of the result, and where its code is 0 only what the
+    offsets' difference leaves of it is."""
+    _attend([2, 17, 7, 16, 7, 20], [43, 17, 269, 17, 142, 41], 2, 1, seed=198495, scale=0.3, max_rows=1, width=11)
+    _attend([2, 17, 7, 16, 7, 20], [43, 17, 269, 17, 142, 41], 8, 1, seed=198496, scale=0.3, max_rows=20)
 
 
 def test_queries_of_any_size():
