@@ -184,14 +184,9 @@ __device__ __forceinline__ void load_turn(const WriteArgs& p, int t, int i, Turn
   unpack4(__ldg(reinterpret_cast<const uint2*>(p.sin + at + 64)), r.sb);
 }
 
-// The codes of one key, lane i's low and high ones, and the scales of its two groups.
-struct KeyCodes {
-  uint32_t lo, hi;
-  float s_lo, s_hi;
-};
-// In fp64, from the inputs.
-__device__ __forceinline__ KeyCodes exact_key(const uint2* x, const uint2* w, const uint2* c, const uint2* s, float eps, int i,
-                                           uint32_t mask) {
+// A head's values after norm and rotation in fp64, from the inputs: lane i's channels 4i.. and 64+4i...
+__device__ __forceinline__ void exact_head(const uint2* x, const uint2* w, const uint2* c, const uint2* s, float eps, int i,
+                                           uint32_t mask, double (&ya)[4], double (&yb)[4]) {
   float xa[4], xb[4], wa[4], wb[4], ca[4], cb[4], sa[4], sb[4];
   unpack4(__ldg(x + i), xa);
   unpack4(__ldg(x + 16 + i), xb);
@@ -201,7 +196,7 @@ __device__ __forceinline__ KeyCodes exact_key(const uint2* x, const uint2* w, co
   unpack4(__ldg(c + 16 + i), cb);
   unpack4(__ldg(s + i), sa);
   unpack4(__ldg(s + 16 + i), sb);
-  double sum = 0.0, ya[4], yb[4];
+  double sum = 0.0;
 #pragma unroll
   for (int e = 0; e < 4; ++e) sum += (double)xa[e] * (double)xa[e] + (double)xb[e] * (double)xb[e];
   const double norm = 1.0 / sqrt(head_sum(sum, mask) / D + (double)eps);
@@ -211,6 +206,57 @@ __device__ __forceinline__ KeyCodes exact_key(const uint2* x, const uint2* w, co
     ya[e] = na * (double)ca[e] - nb * (double)sa[e];
     yb[e] = nb * (double)cb[e] + na * (double)sb[e];
   }
+}
+__device__ __forceinline__ void store_query(uint16_t* dst, const float (&ya)[4], const float (&yb)[4]) {
+  *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(ya[0], ya[1]), pack_bf16(ya[2], ya[3]));
+  *reinterpret_cast<uint2*>(dst + 64) = make_uint2(pack_bf16(yb[0], yb[1]), pack_bf16(yb[2], yb[3]));
+}
+// Whether fp32 holds a query's mean square plus eps, and the squares that count in it.
+constexpr float MOST = 1e33f;
+__device__ __forceinline__ bool in_range(float mean) { return mean > SMALL && mean < MOST; }
+__device__ __forceinline__ const uint2* query_of(const WriteArgs& p, int t, int h) {
+  return reinterpret_cast<const uint2*>(p.qkv + (int64_t)t * p.row_stride + (int64_t)h * D);
+}
+// A query that is not in range (values of 2^55 and more, or tiny ones with an eps as small): in fp64.
+__device__ __forceinline__ void far_query(const WriteArgs& p, int t, int h, int i, uint32_t mask) {
+  double da[4], db[4];
+  float ya[4], yb[4];
+  exact_head(query_of(p, t, h), reinterpret_cast<const uint2*>(p.q_norm), reinterpret_cast<const uint2*>(p.cos + (int64_t)t * D),
+             reinterpret_cast<const uint2*>(p.sin + (int64_t)t * D), p.eps, i, mask, da, db);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    ya[e] = (float)da[e];
+    yb[e] = (float)db[e];
+  }
+  store_query(p.yq + ((int64_t)h * p.seqs.T + t) * D + 4 * i, ya, yb);
+}
+// Those of this half warp's U heads, found again from the inputs: the caller keeps no register for it.
+template <int U>
+__device__ __noinline__ void far_queries(const WriteArgs& p) {
+  const int i = threadIdx.x & 15, t = (int)(blockIdx.z * gridDim.y + blockIdx.y);
+  const int h0 = (int)(blockIdx.x * 2 * WARPS + (threadIdx.x >> 4)) * U;
+  const uint32_t mask = 0xffffu << (threadIdx.x & 16);
+#pragma unroll 1
+  for (int h = h0; h < min(h0 + U, p.HQ); ++h) {
+    const uint2* x = query_of(p, t, h);
+    float xa[4], xb[4], ss = 0.f;
+    unpack4(__ldg(x + i), xa);
+    unpack4(__ldg(x + 16 + i), xb);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ss = fmaf(xa[e], xa[e], fmaf(xb[e], xb[e], ss));
+    if (!in_range(head_sum(ss, mask) * (1.f / D) + p.eps)) far_query(p, t, h, i, mask);
+  }
+}
+
+// The codes of one key, lane i's low and high ones, and the scales of its two groups.
+struct KeyCodes {
+  uint32_t lo, hi;
+  float s_lo, s_hi;
+};
+__device__ __forceinline__ KeyCodes exact_key(const uint2* x, const uint2* w, const uint2* c, const uint2* s, float eps, int i,
+                                           uint32_t mask) {
+  double ya[4], yb[4];
+  exact_head(x, w, c, s, eps, i, mask, ya, yb);
   KeyCodes k;
   k.lo = key_codes(ya, mask, k.s_lo);
   k.hi = key_codes(yb, mask, k.s_hi);
@@ -226,7 +272,7 @@ __device__ __noinline__ KeyCodes exact_key_call(const uint2* x, const uint2* w, 
 
 // U: query heads of a half warp.
 template <int U>
-__global__ void __launch_bounds__(WARPS * 32, U > 1 ? 5 : 4) kv4_write_kernel(const WriteArgs p, int q_chunks) {
+__global__ void __launch_bounds__(WARPS * 32, U > 1 ? 5 : 4) kv4_write_kernel(const __grid_constant__ WriteArgs p, int q_chunks) {
   pdl_wait();
   pdl_launch();
   const int lane = threadIdx.x & 31, i = lane & 15, slot = threadIdx.x >> 4;
@@ -252,6 +298,8 @@ __global__ void __launch_bounds__(WARPS * 32, U > 1 ? 5 : 4) kv4_write_kernel(co
     unpack4(__ldg(reinterpret_cast<const uint2*>(p.q_norm + 4 * i)), wa);
     unpack4(__ldg(reinterpret_cast<const uint2*>(p.q_norm + 64 + 4 * i)), wb);
     if (t < __ldg(p.seqs.row_start) || t >= __ldg(p.seqs.row_start + p.seqs.B)) return;
+    auto query = [&](int u) { return p.yq + ((int64_t)(h0 + u) * p.seqs.T + t) * D + 4 * i; };
+    float means = 0.f;  // looked at once for all heads: a branch a head keeps their arithmetic apart
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (h0 + u >= p.HQ) break;
@@ -260,7 +308,14 @@ __global__ void __launch_bounds__(WARPS * 32, U > 1 ? 5 : 4) kv4_write_kernel(co
       unpack4(ub[u], xb);
 #pragma unroll
       for (int e = 0; e < 4; ++e) ss = fmaf(xa[e], xa[e], fmaf(xb[e], xb[e], ss));
-      const float inv = __frsqrt_rn(head_sum(ss, mask) * (1.f / D) + p.eps);
+      const float mean = head_sum(ss, mask) * (1.f / D) + p.eps;
+      const float inv = __frsqrt_rn(mean);
+      if (U > 1) {
+        means += mean;
+      } else if (!in_range(mean)) {  // before the store: a call of one row may write over its inputs
+        far_query(p, t, h0, i, mask);
+        break;
+      }
       float ya[4], yb[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -268,10 +323,9 @@ __global__ void __launch_bounds__(WARPS * 32, U > 1 ? 5 : 4) kv4_write_kernel(co
         ya[e] = na * r.ca[e] - nb * r.sa[e];
         yb[e] = nb * r.cb[e] + na * r.sb[e];
       }
-      uint16_t* dst = p.yq + ((int64_t)(h0 + u) * p.seqs.T + t) * D + 4 * i;
-      *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(ya[0], ya[1]), pack_bf16(ya[2], ya[3]));
-      *reinterpret_cast<uint2*>(dst + 64) = make_uint2(pack_bf16(yb[0], yb[1]), pack_bf16(yb[2], yb[3]));
+      store_query(query(u), ya, yb);
     }
+    if (U > 1 && !(means < MOST && p.eps > SMALL)) far_queries<U>(p);
     return;
   }
   const int pair = (chunk - q_chunks) * 2 * WARPS + slot;

@@ -1,0 +1,59 @@
+"""Edges of the 4-bit K/V cache on the GPU: values at both ends of what is held."""
+import types
+
+import pytest
+import torch
+
+from fastforward_b200 import _lib as L
+from fastforward_b200 import ops
+from tests import _kv4 as ref
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+DEV = "cuda"
+
+
+@pytest.fixture(autouse=True)
+def _no_device_error():
+    L.device_error(clear=True)
+    yield
+    assert L.device_error(clear=True) == 0
+
+
+def _ints(*x):
+    return torch.tensor(x, dtype=torch.int32)
+
+
+def _norm(seed, eps=1e-6):
+    g = torch.Generator().manual_seed(seed)
+    return types.SimpleNamespace(weight=(1 + 0.2 * torch.randn(128, generator=g)).to(BF16), variance_epsilon=eps)
+
+
+def _dev(x):
+    if isinstance(x, types.SimpleNamespace):
+        return types.SimpleNamespace(weight=x.weight.to(DEV), variance_epsilon=x.variance_epsilon)
+    return x.to(DEV)
+
+
+@pytest.mark.parametrize("rows", [40, 640])
+@pytest.mark.parametrize("eps", [1e-6, 0.0, 1e-30, 3.0])
+def test_written_queries_of_any_size(rows, eps):
+    """Rows from tiny to huge, past where fp32 holds their squares' sum: the queries are the formula's."""
+    hq, hk = 4, 1
+    g = torch.Generator().manual_seed(rows)
+    qkv = (torch.randn(rows, (hq + 2 * hk) * 128, generator=g) * torch.logspace(-37, 37, rows)[:, None]).to(BF16)
+    qkv[7, :128:3] = (qkv[7, :128:3].double() * 2.0 ** -40).to(BF16)
+    angle = torch.rand(rows, 128, generator=g) * 6.3
+    cos, sin = angle.cos().to(BF16), angle.sin().to(BF16)
+    qn, kn = _norm(1, eps), _norm(2, eps)
+    pages = ops.kv4_pages(rows // 64 + 1, hk)
+    table = torch.arange(pages.shape[0], dtype=torch.int32)[None]
+    got = ops.qk_pair_kv4(_dev(qkv), _dev(qn), _dev(kn), _dev(cos), _dev(sin), pages, _dev(table), _dev(_ints(0, rows)),
+                          _dev(_ints(rows))).cpu().double()
+    # eps is a float in the call.  Sixteen roundings of fp32 at most (sum of squares, half of each; root,
+    # products) on each of two terms and one to bf16, of
+    # which the smallest number is 2^-133
+    exact = types.SimpleNamespace(weight=qn.weight, variance_epsilon=float(torch.tensor(eps, dtype=torch.float32)))
+    want = ref.norm_rotate(qkv.double().reshape(rows, -1, 128).transpose(0, 1)[:hq], exact, cos, sin)
+    terms = ref.query_terms(qkv, exact, cos, sin, hq)
+    assert ((got - want).abs() <= want.abs() * 2.0 ** -8 * 1.01 + terms * 2.0 ** -20 + 2.0 ** -134).all()
