@@ -682,9 +682,10 @@ __global__ void __launch_bounds__(THREADS, Shape<NT>::PER_SM) kv4_attention_kern
             pb[n][2 * j] = pack_bf16(y02.x, y13.x);
             pb[n][2 * j + 1] = pack_bf16(y02.y, y13.y);
           }
-          if (masked) {  // nothing of a masked token counts, whatever its scale holds
-            const uint32_t ka = (p[0] == 0.f ? 0u : 0xffffu) | (p[1] == 0.f ? 0u : 0xffff0000u);
-            const uint32_t kb = (p[2] == 0.f ? 0u : 0xffffu) | (p[3] == 0.f ? 0u : 0xffff0000u);
+          if (masked) {  // nothing of a masked token counts, whatever its scale holds; one that is seen counts at p = 0 too
+            const float(&x)[4] = s[f][n];
+            const uint32_t ka = (x[0] == -INFINITY ? 0u : 0xffffu) | (x[1] == -INFINITY ? 0u : 0xffff0000u);
+            const uint32_t kb = (x[2] == -INFINITY ? 0u : 0xffffu) | (x[3] == -INFINITY ? 0u : 0xffff0000u);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               pb[n][2 * j] &= ka;
@@ -868,7 +869,9 @@ __global__ void __launch_bounds__(THREADS, Shape<NT>::PER_SM) kv4_attention_kern
           float2 ml = make_float2(-INFINITY, 0.f);
           if (mine <= me) ml = __ldcg(reinterpret_cast<const float2*>(args.part_ml + pt * 2));
           const float top = fmaxf(s.top, warp_max(ml.x));
-          const float f = ml.x == -INFINITY && ml.y == 0.f ? 0.f : ex2(ml.x - top), fs = s.top == top ? 1.f : ex2(s.top - top);
+          const bool any = !(ml.x == -INFINITY && ml.y == 0.f);  // of the row was seen there
+          const uint32_t seen = __ballot_sync(0xffffffffu, any);
+          const float f = any ? ex2(ml.x - top) : 0.f, fs = s.top == top ? 1.f : ex2(s.top - top);
           s.l = fmaf(s.l, fs, warp_sum(ml.y * f));
           s.o = make_float4(s.o.x * fs, s.o.y * fs, s.o.z * fs, s.o.w * fs);
           s.top = top;
@@ -879,7 +882,7 @@ __global__ void __launch_bounds__(THREADS, Shape<NT>::PER_SM) kv4_attention_kern
             const float4 v = __ldcg(reinterpret_cast<const float4*>(
                 args.part_o + (((int64_t)part * 2 + (part == c_lo)) * QT + col) * D + 4 * lane));
             const float w = __shfl_sync(0xffffffffu, f, i);
-            if (w != 0.f) {  // a part that saw nothing may hold anything
+            if (seen >> i & 1u) {  // a part that saw nothing may hold anything; NaN of no weight is NaN
               s.o.x = fmaf(v.x, w, s.o.x);
               s.o.y = fmaf(v.y, w, s.o.y);
               s.o.z = fmaf(v.z, w, s.o.z);

@@ -1,4 +1,4 @@
-"""Edges of the 4-bit K/V cache on the GPU: values at both ends of what is held."""
+"""Edges of the 4-bit K/V cache on the GPU: values at both ends of what is held, and NaN."""
 import types
 
 import pytest
@@ -35,6 +35,15 @@ def _dev(x):
     return x.to(DEV)
 
 
+def _run(q, pages, table, starts, lens, scale, **kw):
+    return ops.attention_kv4(_dev(q), _dev(pages), _dev(table), _dev(starts), _dev(lens), scale, **kw).cpu()
+
+
+def _kv(num, hk, seed):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(num, hk, 64, 128, generator=g, dtype=torch.float64) for _ in range(2))
+
+
 @pytest.mark.parametrize("rows", [40, 640])
 @pytest.mark.parametrize("eps", [1e-6, 0.0, 1e-30, 3.0])
 def test_written_queries_of_any_size(rows, eps):
@@ -57,3 +66,33 @@ def test_written_queries_of_any_size(rows, eps):
     want = ref.norm_rotate(qkv.double().reshape(rows, -1, 128).transpose(0, 1)[:hq], exact, cos, sin)
     terms = ref.query_terms(qkv, exact, cos, sin, hq)
     assert ((got - want).abs() <= want.abs() * 2.0 ** -8 * 1.01 + terms * 2.0 ** -20 + 2.0 ** -134).all()
+
+
+def _group_nan(pages, page, token, value):
+    """The first scale group of a token of head 0 reads as NaN: its key (value 0) or its value (1)."""
+    at = 8192 + 512 * value + 8 * token
+    pages[page, 0, at:at + 2] = torch.tensor([0xC0, 0x7F], dtype=torch.uint8)
+
+
+@pytest.mark.parametrize("value", [0, 1])
+@pytest.mark.parametrize("rows,n,at,low", [(1, 70, 66, (66, 67)), (1, 70, 3, (3, 4)), (3, 70, 64, (60, 67)),
+                                           (40, 90, 66, (66, 67)), (1, 6000, 100, (0, 1500)), (1, 6000, 4000, (3000, 4500)),
+                                           (40, 6000, 100, (0, 1500))])
+def test_nan_of_no_weight_is_seen(value, rows, n, at, low):
+    """A key or value that reads as NaN, beside keys `low` whose probability is 0 in fp32, its own
+    among them: 0 x NaN is NaN in the rows that see it, whatever page, CTA or kernel it falls to."""
+    num = -(-n // 64)
+    k, v = _kv(num, 1, 3)
+    for j in range(*low):
+        k[j // 64, :, j % 64] = -8.0
+    pages = ref.pack(k, v)
+    _group_nan(pages, at // 64, at % 64, value)
+    q = torch.ones(4, rows, 128).to(BF16)  # scores of the low keys: -1024
+    table = torch.arange(num, dtype=torch.int32)[None]
+    for width in (num, 200):  # narrow: an item a CTA; wide: shared out
+        wide = torch.full((1, max(width, num)), -1, dtype=torch.int32)
+        wide[:, :num] = table
+        got = _run(q, pages, wide, _ints(0, rows), _ints(n), 1.0, max_rows=rows)
+        sees = torch.arange(n - rows, n) >= at
+        assert got[sees][..., :32].isnan().all()
+        assert not got[~sees].isnan().any()
