@@ -500,6 +500,8 @@ def qk_pair_kv4(qkv, qn, kn, cos, sin, pages, page_table, row_start, ctx_len, ou
 def kv4_read(pages, page_table, row_start, ctx_len, rows):
     """The newest rows as the 4-bit cache holds them: k, v [HK, rows, 128] bf16, exact.  To read
     whole sequences, pass row_start with ctx_len's running sums."""
+    if not 0 <= rows <= 1 << 24:
+        _need(False, f"rows {rows} (0 to 2^24)")
     place, dev, b, hk = _kv4_place(pages, page_table, row_start, ctx_len)
     k, v = (pages.new_empty((hk, rows, 128), dtype=BF16) for _ in range(2))
     if rows:
@@ -517,6 +519,8 @@ def attention_kv4(q, pages, page_table, row_start, ctx_len, scale, window=0, sin
     slice of row_start, ctx_len and page_table.
     Held values must be below 2^57 in size.  Returns [T, HQ, 128] bf16 (`out`, or a new tensor; rows
     of no sequence are left as they were)."""
+    if not (0 <= window <= 1 << 30 and 0 <= sinks <= 1 << 30):  # the C call takes 32 bits of them
+        _need(False, f"window {window}, sinks {sinks} (0 to 2^30)")
     place, dev, b, hk = _kv4_place(pages, page_table, row_start, ctx_len)
     if q.dtype is not BF16 or q.get_device() != dev:
         _need(False, "q must be bf16, on the cache's device")
