@@ -70,6 +70,7 @@ constexpr int HALF_BYTES = HALF_VS + HALF_SCALES;
 constexpr int QROW = 2 * D + 16;      // byte pitch of a query row (spreads the banks)
 constexpr int CS = D + 4;             // fp32 pitch of a column in the final exchange (spreads the banks)
 constexpr float LAZY = 8.f;
+constexpr float LOG2E = 1.4426950408889634f;
 constexpr float UNSEEN = 3e38f;       // 64 - maximum before the first score: finite, so that -inf gives exp2(-inf)
 
 constexpr int MIN_PAGES = GROUPS;     // fewest pages worth a CTA: one a group
@@ -1068,7 +1069,7 @@ extern "C" int ffb_attention_kv4(const uint16_t* q, const uint8_t* pages, int nu
   FFB_REQUIRE(q && out, "%s: NULL pointer", who);
   FFB_REQUIRE(HQ > 0 && HQ % HK == 0 && HQ <= 4096, "%s: bad heads HQ=%d HK=%d", who, HQ, HK);
   FFB_REQUIRE(max_rows > 0 && max_rows <= T, "%s: max_rows %d (1..T=%d)", who, max_rows, T);
-  FFB_REQUIRE(isfinite(scale), "%s: scale must be finite", who);
+  FFB_REQUIRE(isfinite(scale * LOG2E), "%s: scale %g (times log2 e it must be finite)", who, (double)scale);
   FFB_REQUIRE(window >= 0 && sinks >= 0 && window <= (1 << 30) && sinks <= (1 << 30), "%s: window %d, sinks %d", who,
               window, sinks);
   FFB_REQUIRE((int64_t)T * HQ <= (1 << 30), "%s: T=%d x HQ=%d too large", who, T, HQ);
@@ -1079,7 +1080,7 @@ extern "C" int ffb_attention_kv4(const uint16_t* q, const uint8_t* pages, int nu
               "%s: workspace of %lld bytes (16-byte aligned) needed, %lld given", who, (long long)p.bytes, (long long)ws_bytes);
   AttnArgs a = {q, out, nullptr, 0, nullptr, nullptr,
                 {const_cast<uint8_t*>(pages), page_table, row_start, ctx_len, num_pages, max_pages, B, T, HK, table_stride},
-                HQ, p.splits, window, sinks, p.whole, p.cut, scale * 1.4426950408889634f, nullptr};
+                HQ, p.splits, window, sinks, p.whole, p.cut, scale * LOG2E, nullptr};
   cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e;
   if (p.kernel == TC) {

@@ -24,3 +24,15 @@ def test_reads_of_rows_that_do_not_fit_are_refused(rows):
     i = torch.zeros(2, dtype=torch.int32)
     with pytest.raises(ValueError, match="rows"):
         ops.kv4_read(pages, i[:1, None], i, i[:1], rows)
+
+
+def _attend(**k):
+    a = dict(q=P, pages=P, num=4, table=P, stride=4, width=4, start=P, ctx=P, out=P + (1 << 20), ws=P, bytes=1 << 40, B=1, T=3,
+             most=1, HQ=4, HK=1, scale=0.1, window=0, sinks=0) | k
+    L.call("ffb_attention_kv4", *a.values(), None)
+
+
+@pytest.mark.parametrize("scale", [3e38, -2.5e38, float("inf"), float("nan")])
+def test_scales_that_overflow_in_base_2_are_refused(scale):
+    with pytest.raises(ValueError, match="scale"):
+        _attend(scale=scale)
