@@ -534,9 +534,10 @@ __global__ void __launch_bounds__(THREADS, Shape<NT>::PER_SM) kv4_attention_kern
       if (t == 0) {
         ssum[(8 * n + g) * 4 + j] = sum * -0x1p-21f;  // -8 x 2^-24
         // scores come out 2^-24 factor times too large; beyond 2^110 the (one-hot) softmax only
-        // needs their order.  Never 0: a masked -inf stays one
+        // needs their order, as with a factor past 2^116.  Never 0: a masked -inf stays one
         if (j == 0)
-          smul[8 * n + g] = fmaxf(fabsf(args.scale_log2) * __uint_as_float((uint32_t)(127 + 10 + min(ex, 110)) << 23), 1e-37f);
+          smul[8 * n + g] = fminf(
+              fmaxf(fabsf(args.scale_log2) * __uint_as_float((uint32_t)(127 + 10 + min(ex, 110)) << 23), 1e-37f), 0x1p116f);
       }
     }
     __syncthreads();
@@ -648,10 +649,19 @@ __global__ void __launch_bounds__(THREADS, Shape<NT>::PER_SM) kv4_attention_kern
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-          if (x == -INFINITY) continue;
-          const float to = fminf(neg[i], 64.f - x * mul[i]), a = ex2(to - neg[i]), nm = 64.f - to;
+          const bool up = x > high[i];
+          const float base = smul[8 * (i >> 1) + 2 * t + (i & 1)];
+          float to = 64.f - x * mul[i], to_mul = mul[i], a = ex2(to - neg[i]);
+          if (fabsf(to) > 0x1p30f || to_mul != base) {  // vast scores, or no longer: an old maximum has no weight beside the new
+            const float small = vast_scale(x * base);
+            to_mul = base * small;
+            to = (small == 1.f ? 64.f : 32.f) - x * to_mul;
+            a = to_mul == mul[i] ? ex2(to - neg[i]) : 0.f;
+          }
+          if (!up) continue;
           neg[i] = to;
-          high[i] = __fdividef(nm + LAZY, mul[i]);
+          mul[i] = to_mul;
+          high[i] = x + __fdividef(LAZY, to_mul);
           l[i] *= a;
 #pragma unroll
           for (int d = 0; d < 8; ++d) {
@@ -779,7 +789,7 @@ __global__ void __launch_bounds__(THREADS, Shape<NT>::PER_SM) kv4_attention_kern
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 16);
       if (g == 0) {
         const int c = 8 * (i >> 1) + 2 * t + (i & 1);
-        xm[warp * QT + c] = neg[i] == UNSEEN ? -INFINITY : 64.f - neg[i];
+        xm[warp * QT + c] = neg[i] == UNSEEN ? -INFINITY : mul[i] == smul[c] ? 64.f - neg[i] : (64.f - neg[i]) * (smul[c] / mul[i]);
         xl[warp * QT + c] = l[i] * 0x1p-64f;
       }
     }

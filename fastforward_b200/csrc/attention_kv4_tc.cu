@@ -471,7 +471,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
       if (x == 0 || two) {
         const uint32_t base_blk = x ? blkB0 : blk0;
         const volatile Work& w = *work;
-        const float sc = fmaxf(fabsf(args.scale_log2), 1e-37f);  // scale 0: a masked -inf stays one
+        const float base = fmaxf(fabsf(args.scale_log2), 1e-37f);  // scale 0: a masked -inf stays one
+        float sc = base;                                           // smaller while the row's scores are vast
         // this thread's column (past the last: the last one's), and its row and head, which shuffles
         // hand on
         auto column = [&] { return min(w.c0 + 128 * x + r, w.clast); };
@@ -510,7 +511,6 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
         const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
         const uint32_t st = tmem + lane_addr + 128 * x, ot = tmem + lane_addr + 256 + 128 * x;
         float m = -INFINITY, neg = 0.f, l = 0.f;  // neg: -m, 0 while nothing has been seen
-        const float2 sc2 = make_float2(sc, sc);
         for (int j = 0; j < nblk; ++j) {
           const bool part = j < w.seen0 || j >= w.seen1;
           if (!__all_sync(0xffffffffu, wait_held(&s_full[x], (base_blk + j) & 1u, abort_flag) && !*abort_flag)) {
@@ -558,11 +558,12 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
           }
           uint32_t w[2][16];  // the scores again, for the probabilities: on their way while the maximum is looked at
           tmem_ld16_async(st, w[0]);
-          const float bmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
-          const bool grow = bmax > m + LAZY;
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          const bool grow = top * sc > m + LAZY;
           if (__any_sync(0xffffffffu, grow)) {
-            const float nm = grow ? bmax : m;
-            const float alpha = grow ? ex2(m - nm) : 1.f;
+            const float to_sc = grow ? base * vast_scale(top * base) : sc, nm = grow ? top * to_sc : m;
+            const float alpha = grow ? (to_sc == sc ? ex2(m - nm) : 0.f) : 1.f;
+            sc = to_sc;
             l *= alpha;
             m = nm;
             neg = m == -INFINITY ? 0.f : -m;
@@ -585,7 +586,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
               tmem_wait_st();
             }
           }
-          const float2 neg2 = make_float2(neg, neg);
+          const float2 neg2 = make_float2(neg, neg), sc2 = make_float2(sc, sc);
           float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
           for (int q = 0; q < 8; ++q) {
@@ -622,7 +623,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
             const int column = 128 * x + r;
             const bool live_row = w.c0 + column <= w.clast;
             float4* to = reinterpret_cast<float4*>(args.part_o) + part * (256 * D / 4) + column;
-            if (live_row) *reinterpret_cast<float2*>(args.part_ml + (part * 256 + column) * 2) = make_float2(m, l);
+            if (live_row)
+              *reinterpret_cast<float2*>(args.part_ml + (part * 256 + column) * 2) = make_float2(sc == base ? m : m * (base / sc), l);
 #pragma unroll 1
             for (int q = 0; q < 4; ++q) {
               uint32_t v[32];

@@ -114,6 +114,14 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// What a row's scores are multiplied with when its maximum (base 2) is m.  Up to 2^30 in size nothing: 1.
+// Beyond, fp32 scores next to each other are 32 and more apart, so that only their order counts, but
+// x mul - m in one rounding may be off by as much as m is, by far more than exp2 holds: a power of two
+// brings m between 2^29 and 2^30, where it is off by 32 at most.
+__device__ __forceinline__ float vast_scale(float m) {
+  const uint32_t e = (__float_as_uint(m) >> 23) & 255u;
+  return e < 127 + 30 ? 1.f : __uint_as_float((127 + 29 + 127 - e) << 23);
+}
 // Nibbles i and i + 4 of w as the bf16 pair (136 + code).
 __device__ __forceinline__ uint32_t pair136(uint32_t w, int i) { return ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u; }
 __device__ __forceinline__ uint32_t minus136(uint32_t w) {

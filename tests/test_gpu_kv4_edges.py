@@ -96,3 +96,30 @@ def test_nan_of_no_weight_is_seen(value, rows, n, at, low):
         sees = torch.arange(n - rows, n) >= at
         assert got[sees][..., :32].isnan().all()
         assert not got[~sees].isnan().any()
+
+
+@pytest.mark.parametrize("rows", [1, 4, 40])
+@pytest.mark.parametrize("scale,size", [(2.0 ** 100, 2.0 ** 20), (2.0 ** 60, 2.0 ** 60), (1.0, 2.0 ** 115), (2.0 ** 120, 1.0),
+                                        (0.7, 2.0 ** 80), (0.09, 2.0 ** 40), (-0.3, 2.0 ** 30), (2.0 ** 25, 1.0)])
+@pytest.mark.parametrize("ctx", [250, 5000])
+@pytest.mark.parametrize("below", [False, True])
+def test_scores_past_what_exp2_can_tell(rows, scale, size, ctx, below):
+    """Scores of 2^25 to 2^123, of both signs or all below 0: next to the best key the others have no
+    weight, so each row is that key's value, whatever queries and scale the size comes from."""
+    num = -(-ctx // 64)
+    k, v = _kv(num, 1, 8)
+    q = torch.randn(4, rows, 128, generator=torch.Generator().manual_seed(5)) * size
+    if below:
+        k, q = k.abs(), -q.abs() if scale > 0 else q.abs()
+    pages, q = ref.pack(k, v), q.to(BF16)
+    got = _run(q, pages, torch.arange(num, dtype=torch.int32)[None], _ints(0, rows), _ints(ctx), scale, max_rows=rows).double()
+    held_k, held_v = (x.reshape(num * 64, 128) for x in ref.unpack(pages))
+    s = q.double() @ held_k.T * scale
+    s.masked_fill_(torch.arange(num * 64) > torch.arange(ctx - rows, ctx)[:, None], -torch.inf)
+    best = s.topk(2, -1)
+    clear = best.values[..., 0] - best.values[..., 1] > 100 + 2.0 ** -15 * best.values[..., 0].abs()  # fp32 products tell them apart
+    assert clear.double().mean() > 0.9
+    want = held_v[best.indices[..., 0]]
+    # the offsets leave 2^-22 255 of the scale of the value's group, below 2^-14 of the row's largest
+    off = (got.transpose(0, 1) - want).abs() <= want.abs() * 2.0 ** -8 * 2.02 + 2.0 ** -14 * want.abs().amax(-1, keepdim=True)
+    assert off[clear].all()
