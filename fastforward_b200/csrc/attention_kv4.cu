@@ -1088,6 +1088,8 @@ extern "C" int ffb_attention_kv4(const uint16_t* q, const uint8_t* pages, int nu
   const Plan p = make_plan(B, T, HQ, HK, max_rows, max_pages, window, sinks);
   FFB_REQUIRE(p.bytes == 0 || (ws && ws_bytes >= p.bytes && ffb::aligned(ws, 16)),
               "%s: workspace of %lld bytes (16-byte aligned) needed, %lld given", who, (long long)p.bytes, (long long)ws_bytes);
+  const int64_t bytes = (int64_t)T * HQ * D * 2;
+  FFB_REQUIRE(((T == 1 || HQ == 1) && out == q) || !ffb::overlap(q, bytes, out, bytes), "%s: q and out overlap", who);
   AttnArgs a = {q, out, nullptr, 0, nullptr, nullptr,
                 {const_cast<uint8_t*>(pages), page_table, row_start, ctx_len, num_pages, max_pages, B, T, HK, table_stride},
                 HQ, p.splits, window, sinks, p.whole, p.cut, scale * LOG2E, nullptr};

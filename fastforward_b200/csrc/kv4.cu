@@ -470,6 +470,9 @@ extern "C" int ffb_qk_norm_rope_kv4(const uint16_t* qkv, int64_t row_stride, con
   FFB_REQUIRE(ffb::aligned(qkv, 8) && ffb::aligned(q_norm, 8) && ffb::aligned(k_norm, 8) && ffb::aligned(cos, 8) &&
                   ffb::aligned(sin, 8) && ffb::aligned(yq, 8),
               "%s: qkv, norms, tables and yq must be 8-byte aligned", who);
+  FFB_REQUIRE((T == 1 && yq == qkv) || !ffb::overlap(yq, (int64_t)T * HQ * D * 2, qkv,
+                                                      ((T - 1) * row_stride + (int64_t)(HQ + 2 * HK) * D) * 2),
+              "%s: yq and qkv overlap", who);
   WriteArgs a = {qkv, row_stride, q_norm, k_norm, cos, sin, yq, eps, HQ,
                  {pages, page_table, row_start, ctx_len, num_pages, max_pages, B, T, HK, table_stride}};
   // with few rows every half warp has one head: 320 rows take 10 us so, and 7000 rows a third less

@@ -177,6 +177,11 @@ __device__ __forceinline__ PageSet pages_of(int pos_lo, int pos_hi, int max_page
 }  // namespace kv4
 
 namespace ffb {
+// Whether n bytes at a and m bytes at b share any (host).
+inline bool overlap(const void* a, int64_t n, const void* b, int64_t m) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + (uint64_t)m && y < x + (uint64_t)n;
+}
 // The argument checks that every kv4 entry shares (host): FFB_OK or FFB_EINVAL with a message.
 int kv4_check(const char* who, const void* pages, const int* table, const int* row_start, const int* ctx_len,
               int num_pages, int64_t table_stride, int max_pages, int B, int T, int HK);

@@ -468,8 +468,8 @@ def qk_pair_kv4(qkv, qn, kn, cos, sin, pages, page_table, row_start, ctx_len, ou
     (HQ + 2 HK) * 128] (any row stride that is a multiple of 4, unit last), cos / sin [T, 128]
     (or [1, T, 128]).  Rows [row_start[b], row_start[b + 1]) are the newest tokens of sequence
     b, whose cache holds ctx_len[b] tokens with them, in the pages of page_table[b].  Returns
-    the queries [HQ, T, 128] (`out`, or a new tensor; rows of no sequence are left as they
-    were).  Norm, rotation and quantisation run in one pass; the queries round once to bf16."""
+    the queries [HQ, T, 128] (`out`, which may be qkv's own memory when T is 1 and must not overlap it
+    otherwise, or a new tensor; rows of no sequence are left as they were).  Norm, rotation and quantisation run in one pass; the queries round once to bf16."""
     place, dev, b, hk = _kv4_place(pages, page_table, row_start, ctx_len)
     qw, kw, eps = qn.weight, kn.weight, qn.variance_epsilon
     if not (qkv.dtype is qw.dtype is kw.dtype is cos.dtype is sin.dtype is BF16):
@@ -517,8 +517,9 @@ def attention_kv4(q, pages, page_table, row_start, ctx_len, scale, window=0, sin
     known (it sizes the launch and changes no result beyond rounding; default T / B, rounded up).
     Single tokens and long chunks are faster in two calls over the same q and out, each with its
     slice of row_start, ctx_len and page_table.
-    Held values must be below 2^57 in size.  Returns [T, HQ, 128] bf16 (`out`, or a new tensor; rows
-    of no sequence are left as they were)."""
+    Held values must be below 2^57 in size.  Returns [T, HQ, 128] bf16 (`out`, which may be q's
+    own memory when T or HQ is 1 and must not overlap it otherwise, or a new tensor; rows of no
+    sequence are left as they were)."""
     if not (0 <= window <= 1 << 30 and 0 <= sinks <= 1 << 30):  # the C call takes 32 bits of them
         _need(False, f"window {window}, sinks {sinks} (0 to 2^30)")
     place, dev, b, hk = _kv4_place(pages, page_table, row_start, ctx_len)

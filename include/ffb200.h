@@ -493,7 +493,8 @@ int ffb_attention_full(const uint16_t* q, const uint16_t* k, const uint16_t* v, 
  * without intermediate bf16 roundings) with the keys and values quantised into the cache in
  * the same pass.  qkv [T, (HQ+2HK)*128] bf16 rows, row_stride elements apart (a multiple of
  * 4); q_norm, k_norm [128]; cos, sin [T, 128] bf16; yq [HQ, T, 128] bf16.  Two rows of a call
- * must not share a position of a page (which of them is held is then not defined). */
+ * must not share a position of a page (which of them is held is then not defined).  yq and qkv must not
+ * overlap, except that yq may be qkv when T is 1. */
 int ffb_qk_norm_rope_kv4(const uint16_t* qkv, int64_t row_stride, const uint16_t* q_norm,
                          const uint16_t* k_norm, float eps, const uint16_t* cos, const uint16_t* sin,
                          uint16_t* yq, uint8_t* pages, int num_pages, const int* page_table,
@@ -506,7 +507,8 @@ int ffb_kv4_read(const uint8_t* pages, int num_pages, const int* page_table, int
                  int T, int HK, void* stream);
 
 /* Causal GQA attention of the rows over their sequences' cached keys (the rows' own among
- * them: write them first).  q [HQ, T, 128], out [T, HQ*128] bf16, 16-byte aligned.  window > 0:
+ * them: write them first).  q [HQ, T, 128], out [T, HQ*128] bf16, 16-byte aligned; they must not overlap,
+ * except that out may be q when T or HQ is 1.  window > 0:
  * row at position p sees keys j <= p with p - j < window or j < sinks; pages that no row sees
  * are not read.  window 0: every key j <= p (sinks must be 0).  A row that sees no key gets
  * zeros; one that sees a NaN key becomes NaN, one that sees a NaN value is NaN in that group of

@@ -123,3 +123,40 @@ def test_scores_past_what_exp2_can_tell(rows, scale, size, ctx, below):
     # the offsets leave 2^-22 255 of the scale of the value's group, below 2^-14 of the row's largest
     off = (got.transpose(0, 1) - want).abs() <= want.abs() * 2.0 ** -8 * 2.02 + 2.0 ** -14 * want.abs().amax(-1, keepdim=True)
     assert off[clear].all()
+
+
+def test_outputs_in_place_of_their_inputs():
+    """One row, or one head: the layouts of queries and result agree and the result may replace them."""
+    k, v = _kv(60, 2, 5)
+    pages, table = ref.pack(k, v), torch.arange(60, dtype=torch.int32)[None]
+    g = torch.Generator().manual_seed(1)
+    for hq, rows, hk in ((8, 1, 2), (96, 1, 2), (1, 20, 1), (1, 300, 1)):
+        q = _dev(torch.randn(hq, rows, 128, generator=g).to(BF16))
+        place = (_dev(pages[:, :hk].contiguous()), _dev(table), _dev(_ints(0, rows)), _dev(_ints(3800)))
+        want = ops.attention_kv4(q, *place, 0.1)
+        got = ops.attention_kv4(q, *place, 0.1, out=q.view(rows, hq, 128))
+        assert got.data_ptr() == q.data_ptr() and torch.equal(got, want)
+    q = _dev(torch.randn(4, 6, 128, generator=g).to(BF16))
+    with pytest.raises(ValueError, match="overlap"):
+        ops.attention_kv4(q, *place[:2], _dev(_ints(0, 6)), place[3], 0.1, out=q.view(6, 4, 128))
+    both = torch.zeros(4 * 6 * 128 + 64, dtype=BF16, device=DEV)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.attention_kv4(both[:-64].view(4, 6, 128), *place[:2], _dev(_ints(0, 6)), place[3], 0.1, out=both[64:].view(6, 4, 128))
+
+
+def test_written_queries_in_place_of_one_row():
+    g = torch.Generator().manual_seed(2)
+    cos, sin = (_dev(torch.rand(3, 128, generator=g).to(BF16)) for _ in range(2))
+    qn, kn = _dev(_norm(1)), _dev(_norm(2))
+    for rows in (1, 3):
+        qkv = _dev(torch.randn(rows, 8 * 128, generator=g).to(BF16))
+        pages = [ops.kv4_pages(1, 2) for _ in range(2)]
+        place = (_dev(_ints(0))[None], _dev(_ints(0, rows)), _dev(_ints(rows)))
+        want = ops.qk_pair_kv4(qkv, qn, kn, cos[:rows], sin[:rows], pages[0], *place)
+        into = qkv.view(-1)[:4 * rows * 128].view(4, rows, 128)
+        if rows == 1:
+            got = ops.qk_pair_kv4(qkv, qn, kn, cos[:rows], sin[:rows], pages[1], *place, out=into)
+            assert torch.equal(got, want) and torch.equal(*pages)
+        else:
+            with pytest.raises(ValueError, match="overlap"):
+                ops.qk_pair_kv4(qkv, qn, kn, cos[:rows], sin[:rows], pages[1], *place, out=into)

@@ -36,3 +36,19 @@ def _attend(**k):
 def test_scales_that_overflow_in_base_2_are_refused(scale):
     with pytest.raises(ValueError, match="scale"):
         _attend(scale=scale)
+
+
+def _write(**k):
+    a = dict(qkv=P, row_stride=768, qn=P, kn=P, eps=1e-6, cos=P, sin=P, yq=P + (1 << 20), pages=P, num=4, table=P, stride=4,
+             width=4, start=P, ctx=P, B=1, T=3, HQ=4, HK=1) | k
+    L.call("ffb_qk_norm_rope_kv4", *a.values(), None)
+
+
+@pytest.mark.parametrize("f,bad", [
+    (_attend, dict(out=P)), (_attend, dict(out=P + 3 * 4 * 256 - 16)), (_attend, dict(out=P - 3 * 4 * 256 + 16)),
+    (_attend, dict(T=1, out=P + 16)), (_attend, dict(HQ=1, out=P + 16)), (_write, dict(yq=P)), (_write, dict(yq=P + 256)),
+    (_write, dict(T=1, yq=P + 8)), (_write, dict(yq=P + (2 * 768 + 6 * 128) * 2 - 8)), (_write, dict(yq=P - 3 * 4 * 256 + 8))])
+def test_overlapping_results_are_refused(f, bad):
+    """A CTA stores its rows while others have yet to read theirs."""
+    with pytest.raises(ValueError, match="overlap"):
+        f(**bad)
