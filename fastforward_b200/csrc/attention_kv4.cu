@@ -770,18 +770,11 @@ __global__ void __launch_bounds__(THREADS, Shape<NT>::PER_SM) kv4_attention_kern
     }
     if (!ok) *abort_flag = 1;
     // a share with fewer pages than stages leaves some of the ring's to fill
-    for (; ahead < min(next_cnt, STAGES) && !*abort_flag; ++ahead)
+    for (; ahead < min(next_cnt, STAGES) && !__any_sync(0xffffffffu, *abort_flag); ++ahead)
       load(__shfl_sync(0xffffffffu, next_ids, ahead), next_head);
     issued = ahead;
     ids = next_ids;
     ids_at = 0;
-    if (lane == 0 && *abort_flag) {  // copies in flight must land before the CTA leaves
-      volatile int never = 0;
-      for (int i = 0; i < STAGES; ++i) {
-        mbar_wait_bounded(full + warp * STAGES + i, 0, &never, 20000000ull);
-        mbar_wait_bounded(full + warp * STAGES + i, 1, &never, 20000000ull);
-      }
-    }
 #pragma unroll
     for (int i = 0; i < 2 * NT; ++i) {
       l[i] += __shfl_xor_sync(0xffffffffu, l[i], 4);
@@ -847,6 +840,16 @@ __global__ void __launch_bounds__(THREADS, Shape<NT>::PER_SM) kv4_attention_kern
       else st_release_gpu_u64(args.flags + 2 * blockIdx.x + (i0 == 0), args.tag);
     }
     turn ^= 1;
+  }
+  copies_done();
+  // A wait that gave up: every warp's copies in flight land before the CTA leaves, those of the warps that
+  // had loaded the next share's first pages by then too.  (The flag is the same for all since the last barrier.)
+  if (lane == 0 && *abort_flag) {
+    volatile int never = 0;
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_wait_bounded(full + warp * STAGES + i, 0, &never, 20000000ull);
+      mbar_wait_bounded(full + warp * STAGES + i, 1, &never, 20000000ull);
+    }
   }
   if (!WHOLE && !__syncthreads_or(*abort_flag) && run.cut.b >= 0) {
     const Share& cut = run.cut;

@@ -297,14 +297,6 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
             mbar_arrive(&raw_full[s]);
           }
         }
-        // the copies have landed before this thread leaves (also when another role gave up)
-        volatile int never = 0;
-        if (*abort_flag) {
-          for (uint32_t i = 0; i < RAW; ++i) {
-            mbar_wait_bounded(&raw_full[i], 0, &never, 20000000ull);
-            mbar_wait_bounded(&raw_full[i], 1, &never, 20000000ull);
-          }
-        }
       }
     } else if (warp == 1) {
       // ---------------------------------------------------------------- MMAs
@@ -694,7 +686,13 @@ __global__ void __launch_bounds__(THREADS, 1) kv4_attention_tc_kernel(const Attn
   }
   tc_fence_before();
   __syncthreads();
-  if (tid == 0 && *abort_flag) atomicOr(args.errors, (uint32_t)ffb::ERR_ATTN_TIMEOUT);
+  if (tid == 0 && *abort_flag) {  // some role gave up (which the roles' last barrier has settled)
+    atomicOr(args.errors, (uint32_t)ffb::ERR_ATTN_TIMEOUT);
+    // pages in flight land before the CTA leaves: the producer may have ended before the others gave up
+    volatile int never = 0;
+#pragma unroll 1
+    for (uint32_t i = 0; i < 2 * RAW; ++i) mbar_wait_bounded(&raw_full[i >> 1], i & 1u, &never, 20000000ull);
+  }
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
