@@ -113,7 +113,7 @@ struct Share {
 // shares of this turn and the next; the first share, if it ends an item that began in another CTA.
 struct Run {
   int64_t left;
-  int b, item, from, more, items, known;
+  int b, item, from, more, items, known, failed;
   Seq seq;
   Share share[2], cut;
 };
@@ -241,6 +241,8 @@ __device__ __forceinline__ void store_row(uint16_t* out, const Sum& s, int lane)
   *reinterpret_cast<uint2*>(out + 4 * lane) = make_uint2(pack_bf16(s.o.x * r, s.o.y * r), pack_bf16(s.o.z * r, s.o.w * r));
 }
 
+// What a call whose wait gave up leaves behind the flags (tags are odd: none is another call's).
+__device__ __forceinline__ uint64_t failed_tag(uint64_t tag) { return tag ^ 1u; }
 // a b / c, in 32 bits where that is enough (a 64-bit division takes hundreds of cycles).
 __device__ __forceinline__ int64_t mul_div(int a, int64_t b, int c) {
   if (b < (1 << 22) && a < 1024) return (uint32_t)a * (uint32_t)b / (uint32_t)c;
@@ -478,6 +480,8 @@ __global__ void __launch_bounds__(THREADS, Shape<NT>::PER_SM) kv4_attention_kern
   };
 
   __syncthreads();
+  // a replay of a call that gave up may find tags of that run: it gives up too
+  if (!WHOLE && tid == 64) run.failed = __ldcg(args.flags + 2 * gridDim.x) == failed_tag(args.tag);
   if (tid == 0) {
     run.cut.b = -1;
     run.known = 0;
@@ -867,7 +871,7 @@ __global__ void __launch_bounds__(THREADS, Shape<NT>::PER_SM) kv4_attention_kern
         }
       }
     }
-    ready = __all_sync(0xffffffffu, ready);
+    ready = __all_sync(0xffffffffu, ready) && !run.failed;
     if (!ready) *abort_flag = 1;
     // `side` warps a column, each with every side-th part: a lane finds a part's weight, then the rows
     // are read with nothing in between
@@ -922,7 +926,10 @@ __global__ void __launch_bounds__(THREADS, Shape<NT>::PER_SM) kv4_attention_kern
     __syncthreads();
     for (int c = c_lo + tid; c < me; c += THREADS) args.flags[2 * c + (c == c_lo)] = 0;
   }
-  if (tid == 0 && *abort_flag) atomicOr(&ffb_device_error_word, (uint32_t)ffb::ERR_ATTN_TIMEOUT);
+  if (tid == 0 && *abort_flag) {
+    atomicOr(&ffb_device_error_word, (uint32_t)ffb::ERR_ATTN_TIMEOUT);
+    if (!WHOLE) args.flags[2 * gridDim.x] = failed_tag(args.tag);
+  }
 }
 
 // Joins the shares of attention_kv4_tc.cu: 16 CTAs an item that was cut, 32 rows and 64 channels each.
@@ -1035,7 +1042,7 @@ Plan make_plan(int B, int T, int HQ, int HK, int max_rows, int max_pages, int wi
     p.splits = pages <= (B * HK * tiles >= 64 ? 32 : 16) ? 1 : 0;
     p.cut = p.whole = 0;
     p.ctas = p.splits ? B * HK : sms * (p.kernel == 1 ? Shape<1>::PER_SM : Shape<2>::PER_SM);
-    p.bytes = p.splits ? 0 : (int64_t)p.ctas * 2 * (8 + width * (D + 2) * 4);
+    p.bytes = p.splits ? 0 : (int64_t)p.ctas * 2 * (8 + width * (D + 2) * 4) + 128;
   }
   return p;
 }
@@ -1106,10 +1113,12 @@ extern "C" int ffb_attention_kv4(const uint16_t* q, const uint8_t* pages, int nu
     e = kv4::launch_attention_tc(a, (unsigned)p.ctas, st);
     if (e == cudaSuccess && p.cut > 0) e = ffb::launch(kv4_join_tc_kernel, dim3((unsigned)p.cut * 16), dim3(256), 0, st, a);
   } else {
-    if (!p.splits) {  // flags, partial rows, their maxima and sums
+    // flags and the mark of a failed run (128 bytes, so that rows stay on their lines: off them 131001 tokens take 50.5 us instead of
+    // 48.3), partial rows, their maxima and sums
+    if (!p.splits) {
       a.flags = static_cast<uint64_t*>(ws);
       a.tag = call_tag();
-      a.part_o = reinterpret_cast<float*>(a.flags + 2 * p.ctas);
+      a.part_o = reinterpret_cast<float*>(a.flags + 2 * p.ctas + 16);
       a.part_ml = a.part_o + (int64_t)p.ctas * 2 * 8 * p.kernel * D;
     }
     e = p.kernel == 1 ? launch_registers<1>(p, a, st) : launch_registers<2>(p, a, st);

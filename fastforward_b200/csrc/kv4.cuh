@@ -63,7 +63,7 @@ __device__ __forceinline__ uint8_t* record_of(const Seqs& s, int b, int64_t pos,
 struct AttnArgs {
   const uint16_t* q;  // [HQ, T, 128]
   uint16_t* out;      // [T, HQ, 128]
-  uint64_t* flags;    // [CTAs][2]: `tag` once that part is written (register path, equal runs)
+  uint64_t* flags;    // [CTAs][2]: `tag` once that part is written (register path, equal runs); behind them a failed run's mark
   uint64_t tag;
   float* part_o;      // partial rows of 128, relative to their maxima: register path [CTAs][2][columns], TC [cut][splits][256]
   float* part_ml;     // their (maximum, sum) pairs

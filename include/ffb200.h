@@ -515,7 +515,9 @@ int ffb_kv4_read(const uint8_t* pages, int num_pages, const int* page_table, int
  * channels at least.  Held values must be below 2^57 in size.  max_rows: the most rows that a
  * sequence has in this call (1..T); it sizes the grid, longer sequences are still computed, only
  * slower.  ws: ffb_attention_kv4_workspace(...) bytes, 16-byte aligned (NULL when 0), scratch of
- * this call alone. */
+ * this call alone.  A captured call that set bit 2 of the device error word (a wait gave up) sets it
+ * again in every later replay on that workspace, without joining the parts of the failed run: capture
+ * it anew. */
 int ffb_attention_kv4(const uint16_t* q, const uint8_t* pages, int num_pages, const int* page_table,
                       int64_t table_stride, int max_pages, const int* row_start, const int* ctx_len,
                       uint16_t* out, void* ws, int64_t ws_bytes, int B, int T, int max_rows, int HQ, int HK,
