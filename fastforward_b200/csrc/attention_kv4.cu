@@ -33,7 +33,8 @@
 //     sum_group 8 s_group sum(q), is one more MMA of the scales themselves with 8 sum(q) in three
 //     bf16 parts, which the scores start from;
 //   - V: probabilities are held 2^64 times too large (so that products with the subnormals are
-//     normal numbers; |v| must stay below 2^57), V's scale multiplies one before its only rounding
+//     normal numbers; |v| must stay below 2^57, and a sum, held 2^-69 too small, is exact to 2^-80: bf16's
+//     bits down to about 2^-68), V's scale multiplies one before its only rounding
 //     to bf16, once per group of channels; movmatrix turns the scores' layout into that of the
 //     second product's operand.  A second MMA with the constants -8 2^-133 and -128 2^-133 takes
 //     the 8 off (half the tensor work, but no instruction a code);

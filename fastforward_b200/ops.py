@@ -514,7 +514,9 @@ def attention_kv4(q, pages, page_table, row_start, ctx_len, scale, window=0, sin
     returns it (the rows' own keys are in the cache already); page_table, row_start, ctx_len as
     there.  window > 0: a row at position p sees keys p - window + 1 .. p and the first `sinks`.
     A row that sees nothing gets zeros.  max_rows: the most rows of one sequence in this call, if
-    known (it sizes the launch and changes no result beyond rounding; default T / B, rounded up).
+    known (it sizes the launch and changes no result beyond rounding; default T / B, rounded up).  Up to
+    32 columns, max_rows HQ / HK, results are held to 2^-79, so that values below about 2^-60 in size lose
+    bits there.
     Single tokens and long chunks are faster in two calls over the same q and out, each with its
     slice of row_start, ctx_len and page_table.
     Held values must be below 2^57 in size.  Returns [T, HQ, 128] bf16 (`out`, which may be q's

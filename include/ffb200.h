@@ -512,9 +512,11 @@ int ffb_kv4_read(const uint8_t* pages, int num_pages, const int* page_table, int
  * row at position p sees keys j <= p with p - j < window or j < sinks; pages that no row sees
  * are not read.  window 0: every key j <= p (sinks must be 0).  A row that sees no key gets
  * zeros; one that sees a NaN key becomes NaN, one that sees a NaN value is NaN in that group of
- * channels at least.  Held values must be below 2^57 in size.  max_rows: the most rows that a
- * sequence has in this call (1..T); it sizes the grid, longer sequences are still computed, only
- * slower.  ws: ffb_attention_kv4_workspace(...) bytes, 16-byte aligned (NULL when 0), scratch of
+ * channels at least.  Held values must be below 2^57 in size, scores and sums within fp32.  max_rows: the
+ * most rows that a sequence has in this call (1..T); it sizes the grid, longer sequences are still
+ * computed, only slower, and it picks the kernel: up to 32 columns, max_rows HQ / HK, results are held
+ * to 2^-79, so that values below about 2^-60 lose bits; with more, values count in full down to the
+ * 2^-100 that the cache holds.  ws: ffb_attention_kv4_workspace(...) bytes, 16-byte aligned (NULL when 0), scratch of
  * this call alone.  A captured call that set bit 2 of the device error word (a wait gave up) sets it
  * again in every later replay on that workspace, without joining the parts of the failed run: capture
  * it anew. */

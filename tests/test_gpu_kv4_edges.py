@@ -7,6 +7,7 @@ import torch
 from fastforward_b200 import _lib as L
 from fastforward_b200 import ops
 from tests import _kv4 as ref
+from tests import _kv4_bounds as bounds
 
 pytestmark = pytest.mark.gpu
 BF16 = torch.bfloat16
@@ -160,3 +161,19 @@ def test_written_queries_in_place_of_one_row():
         else:
             with pytest.raises(ValueError, match="overlap"):
                 ops.qk_pair_kv4(qkv, qn, kn, cos[:rows], sin[:rows], pages[1], *place, out=into)
+
+
+@pytest.mark.parametrize("rows", [1, 4, 40])
+@pytest.mark.parametrize("power", [-90, -62, -40, 40, 54])
+@pytest.mark.parametrize("ctx", [70, 5000])
+def test_values_at_both_ends_of_the_range(rows, power, ctx):
+    """Values from the largest that attention takes to the smallest that the cache holds, through both kernels:
+    the one for few columns holds its sums to 2^-80 only."""
+    num = -(-ctx // 64)
+    k, v = _kv(num, 2, power + 100)
+    v = v.clamp(-3.5, 3.5) * 2.0 ** power  # below 2^57, above 2^-100 for the most part
+    pages, table = ref.pack(k, v), torch.arange(num, dtype=torch.int32)[None]
+    q = torch.randn(8, rows, 128, generator=torch.Generator().manual_seed(2)).to(BF16)
+    got = _run(q, pages, table, _ints(0, rows), _ints(ctx), 0.1, max_rows=rows).double()
+    want, limit = bounds.attention(q, pages, table, _ints(0, rows), _ints(ctx), 0.1, registers=rows * 4 <= 32)
+    assert ((got - want).abs() <= limit).all()
