@@ -1077,6 +1077,9 @@ extern "C" int64_t ffb_attention_kv4_workspace(int B, int T, int HQ, int HK, int
                                                int sinks) {
   if (B <= 0 || T <= 0 || HQ <= 0 || HK <= 0 || HQ % HK != 0 || max_rows <= 0 || max_pages <= 0 || window < 0 || sinks < 0)
     return 0;
+  if (B > 65535 || T > (1 << 24) || HK > 1024 || HQ > 4096 || (int64_t)T * HQ > (1 << 30) || max_rows > T ||
+      max_pages > FFB_KV4_MAX_PAGES || window > (1 << 30) || sinks > (1 << 30))
+    return 0;  // what the call refuses: the plan's products are made for less
   return make_plan(B, T, HQ, HK, max_rows, max_pages, window, sinks).bytes;
 }
 

@@ -524,6 +524,7 @@ int ffb_attention_kv4(const uint16_t* q, const uint8_t* pages, int num_pages, co
                       int64_t table_stride, int max_pages, const int* row_start, const int* ctx_len,
                       uint16_t* out, void* ws, int64_t ws_bytes, int B, int T, int max_rows, int HQ, int HK,
                       float scale, int window, int sinks, void* stream);
+/* Bytes of the workspace; 0 also for shapes that the call refuses. */
 int64_t ffb_attention_kv4_workspace(int B, int T, int HQ, int HK, int max_rows, int max_pages, int window,
                                     int sinks);
 

@@ -52,3 +52,15 @@ def test_overlapping_results_are_refused(f, bad):
     """A CTA stores its rows while others have yet to read theirs."""
     with pytest.raises(ValueError, match="overlap"):
         f(**bad)
+
+
+@pytest.mark.parametrize("at,value", [(0, 65536), (1, 1 << 25), (1, 1 << 30), (2, 4104), (3, 1 << 30), (4, 65), (5, (1 << 24) + 1),
+                                      (6, (1 << 30) + 1), (7, (1 << 30) + 1)])
+def test_workspace_of_refused_shapes_is_zero(at, value):
+    f = L.lib().ffb_attention_kv4_workspace
+    shape = [2, 64, 32, 8, 64, 4096, 1 << 20, 4]
+    assert f(*shape) > 0
+    shape[at] = value
+    if at == 3:
+        shape[2] = value
+    assert f(*shape) == 0
