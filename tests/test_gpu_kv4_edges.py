@@ -1,4 +1,5 @@
-"""Edges of the 4-bit K/V cache on the GPU: values at both ends of what is held, and NaN."""
+"""Edges of the 4-bit K/V cache on the GPU: values at both ends of what is held, NaN, absent
+pages in every schedule, and each kernel within a bound of its own arithmetic."""
 import types
 
 import pytest
@@ -177,3 +178,102 @@ def test_values_at_both_ends_of_the_range(rows, power, ctx):
     got = _run(q, pages, table, _ints(0, rows), _ints(ctx), 0.1, max_rows=rows).double()
     want, limit = bounds.attention(q, pages, table, _ints(0, rows), _ints(ctx), 0.1, registers=rows * 4 <= 32)
     assert ((got - want).abs() <= limit).all()
+
+
+@pytest.mark.parametrize("rows,hq,hk,ctx,width,hint", [
+    (1, 8, 2, [250], 4, 1),                        # an item a CTA
+    (1, 8, 2, [3000, 2000, 1500], 60, 1),          # equal runs that cut the items
+    (3, 8, 2, [4000, 64, 900], 70, 3),
+    (1, 8, 2, [250, 300, 260, 200], 60, 1),        # items apart in a wide table
+    (40, 8, 2, [2500], 40, 40),                    # tcgen05, in shares
+    (20, 16, 2, [700, 130, 64, 900], 16, 20),
+    (80, 96, 24, [400, 300, 500, 200], 9, 80),     # tcgen05, whole items and shares
+    (70, 8, 2, [600, 200], 12, 9),                 # more items than the launch was sized for
+])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (300, 70)])
+def test_absent_pages_in_every_schedule(rows, hq, hk, ctx, width, hint, window, sinks):
+    """Ids outside the cache, in both halves of a block of two pages and in first and last pages of items:
+    their keys are left out.  The ids point just past the slice that the call is given, where
+    pages of NaN lie."""
+    b = len(ctx)
+    need = [-(-c // 64) for c in ctx]
+    num = sum(need)
+    k, v = _kv(num, hk, rows + b)
+    pages = ref.pack(k, v)
+    table = torch.full((b, width), num + 1, dtype=torch.int32)
+    order = torch.randperm(num, generator=torch.Generator().manual_seed(rows)).to(torch.int32)
+    at = 0
+    for i, n in enumerate(need):
+        table[i, :n] = order[at:at + n]
+        at += n
+        absent = {2: [0], 1: []}.get(n, [2, 3] if n < 6 else [0, 3, 6, 7, n - 2] + list(range(9, n - 3, 5)))
+        for j in absent:
+            if j < n - 1:
+                table[i, j] = [num, -1, num + 2, -2 ** 31, 2 ** 31 - 1][j % 5]
+    if b > 1:
+        table[1, need[1] - 1] = num  # the newest keys
+    starts, lens = torch.arange(b + 1, dtype=torch.int32) * rows, _ints(*ctx)
+    q = torch.randn(hq, b * rows, 128, generator=torch.Generator().manual_seed(7)).to(BF16)
+    more = torch.cat([pages, torch.full((4, hk, L.KV4_RECORD), 0xFF, dtype=torch.uint8)])
+    got = ops.attention_kv4(_dev(q), _dev(more)[:num], _dev(table), _dev(starts), _dev(lens), 0.1, window=window, sinks=sinks,
+                            max_rows=hint).cpu().double()
+    assert L.device_error(clear=True) == 1 << 5
+    want, limit = bounds.attention(q, pages, table, starts, lens, 0.1, window, sinks, registers=hint * hq // hk <= 32)
+    assert ((got - want).abs() <= limit).all()
+
+
+@pytest.mark.parametrize("rows,ctx,hint", [(1, 200, 1), (1, 5000, 1), (40, 200, 40), (40, 5000, 40), (150, 2600, 9)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (200, 3)])
+def test_contexts_past_the_table(rows, ctx, hint, window, sinks):
+    """Positions from the table's width on are left out, whole rows among them."""
+    for held in (ctx // 2, ctx - 65):
+        if held < 64:
+            continue
+        num = held // 64
+        k, v = _kv(num, 2, rows)
+        pages, table = ref.pack(k, v), torch.arange(num, dtype=torch.int32)[None]
+        q = torch.randn(8, rows, 128, generator=torch.Generator().manual_seed(3)).to(BF16)
+        more = torch.cat([_dev(table), torch.zeros(1, 400, dtype=torch.int32, device=DEV)], 1)[:, :num]
+        got = ops.attention_kv4(_dev(q), _dev(pages), more, _dev(_ints(0, rows)), _dev(_ints(ctx)), 0.1, window=window,
+                                sinks=sinks, max_rows=hint).cpu().double()
+        assert L.device_error(clear=True) == 1 << 5
+        want, limit = bounds.attention(q, pages, table, _ints(0, rows), _ints(ctx), 0.1, window, sinks, registers=hint * 4 <= 32)
+        assert ((got - want).abs() <= limit).all()
+
+
+@pytest.mark.parametrize("rows,hq,hk,ctx,hint", [
+    (1, 4, 2, [40000], 1), (4, 16, 2, [9000, 30], 4), (1, 300, 1, [500, 70], 1), (1, 1, 1, [20000] * 3, 1),
+    (40, 8, 2, [9000], 40), (300, 4, 4, [700, 3000], 300), (33, 1, 1, [33, 6000], 33)])
+def test_each_kernel_within_its_own_bound(rows, hq, hk, ctx, hint):
+    """Long contexts, where the sums' own rounding counts, and wide groups; the kernel of more than 32
+    columns multiplies values without an offset and is held to that."""
+    need = [-(-c // 64) for c in ctx]
+    k, v = _kv(sum(need), hk, 17)
+    pages = ref.pack(k, v + 0.5)  # sums that grow
+    table = torch.zeros(len(ctx), max(need), dtype=torch.int32)
+    at = 0
+    for i, n in enumerate(need):
+        table[i, :n] = torch.arange(at, at + n)
+        at += n
+    starts, lens = torch.arange(len(ctx) + 1, dtype=torch.int32) * rows, _ints(*ctx)
+    q = torch.randn(hq, len(ctx) * rows, 128, generator=torch.Generator().manual_seed(4)).to(BF16)
+    got = _run(q, pages, table, starts, lens, 0.088, max_rows=hint).double()
+    want, limit = bounds.attention(q, pages, table, starts, lens, 0.088, registers=hint * hq // hk <= 32)
+    assert ((got - want).abs() <= limit).all()
+
+
+def test_a_write_of_more_rows_than_a_grid_is_high():
+    """70000 rows: the launch's rows need its third dimension."""
+    rows = 70000
+    g = torch.Generator().manual_seed(1)
+    qkv = torch.randn(rows, 3 * 128, generator=g).to(BF16)
+    angle = torch.rand(rows, 128, generator=g) * 6.3
+    cos, sin = angle.cos().to(BF16), angle.sin().to(BF16)
+    qn, kn = _norm(1), _norm(2)
+    pages = ops.kv4_pages(-(-rows // 64), 1)
+    place = (torch.arange(pages.shape[0], dtype=torch.int32, device=DEV).flip(0)[None].contiguous(), _dev(_ints(0, rows)), _dev(_ints(rows)))
+    yq = ops.qk_pair_kv4(_dev(qkv), _dev(qn), _dev(kn), _dev(cos), _dev(sin), pages, *place).cpu().double()
+    gk, gv = (x.cpu().double() for x in ops.kv4_read(pages, *place, rows))
+    q, k, v = ref.norm_rotate_quantize(qkv, qn, kn, cos, sin, 1, 1)
+    assert torch.equal(gk, k) and torch.equal(gv, v)
+    assert ((yq - q).abs() <= q.abs() * 2.0 ** -8 * 1.01 + ref.query_terms(qkv, qn, cos, sin, 1) * 2.0 ** -20).all()
