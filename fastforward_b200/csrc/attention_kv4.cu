@@ -100,6 +100,23 @@ __device__ __forceinline__ Seq seq_at(const AttnArgs& a, int b, int qt) {
   q.ps = pages_of(q.ctx - q.S, q.ctx - 1, s.max_pages, a.window, a.sinks);
   return q;
 }
+// The first sequence after b, which has no rows, that has some; B if there is none.  Row starts ascend, so a
+// thousand empty sequences cost a few loads (one after the other they took 150 us).
+__device__ __forceinline__ int next_with_rows(const Seqs& s, int b) {
+  const int end = __ldg(s.row_start + b + 1);
+  int step = 1;
+  while (b + step < s.B && __ldg(s.row_start + b + step + 1) <= end) {
+    b += step;
+    step *= 2;
+  }
+  int lo = b, hi = min(b + step, s.B);  // lo has no rows, hi has or is B
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (__ldg(s.row_start + mid + 1) <= end) lo = mid;
+    else hi = mid;
+  }
+  return hi;
+}
 // One item's share, in shared memory: pages [i0, i1) of sequence b's list `ps` for one K/V head and
 // the columns [c0, clast]; what every warp needs to know about it, found once by one thread.
 struct Share {
@@ -392,7 +409,9 @@ __global__ void __launch_bounds__(THREADS, Shape<NT>::PER_SM) kv4_attention_kern
       while (left > 0 && !more) {
         if (!run.known || item >= run.items) {
           if (run.known) {
-            ++run.b;
+            run.b = run.items > 0 ? run.b + 1 : next_with_rows(sv, run.b);
+            if (run.b >= sv.B) left = 0;  // (row_start does not ascend)
+            if (left == 0) break;
             item = 0;
             from = -ITEM_PAGES;
           }

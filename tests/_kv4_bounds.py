@@ -19,6 +19,7 @@ def attention(q, pages, table, starts, lens, scale, window=0, sinks=0, registers
         largest, which is at most sum |q k|: 136 2^-23 sum |q k|.
       - Scores, registers: codes carry an offset, code + 8 <= 15, whose 8 sum(q) is taken off again: per
         group of channels two MMAs and the subtraction, 2^-21 23 sum_group s_group sum |q| in all.
+      - A probability below 2^-126 of the largest may be 0: exp2 has no subnormals.
       - A score off by e moves a probability by e of itself, the result by e (sum p |v| + |o|).
       - P V, more columns: eight MMAs a block of 128 keys, each cutting 17 terms at 2^-23 of the
         largest, at most sum p |v|: 136 2^-23 sum p |v| a block.
@@ -62,6 +63,7 @@ def attention(q, pages, table, starts, lens, scale, window=0, sinks=0, registers
         else:
             score = 136 * CUT * abs(scale) * torch.where(seen, x.abs() @ k.abs().transpose(1, 2), 0.0)
             product = 136 * CUT * -(-held // 128) * spread
+        product = product + 2.0 ** -126 * (seen.double() @ v.abs()).transpose(0, 1)
         off = score.amax(-1).transpose(0, 1)[..., None]
         limit[r0:r1] += spread * (2.0 ** -8 + 2.0 ** -15) + (spread + o.abs()) * off + product + o.abs() * 2.0 ** -8
         limit[r0:r1] *= 1.01  # products of these

@@ -277,3 +277,26 @@ def test_a_write_of_more_rows_than_a_grid_is_high():
     q, k, v = ref.norm_rotate_quantize(qkv, qn, kn, cos, sin, 1, 1)
     assert torch.equal(gk, k) and torch.equal(gv, v)
     assert ((yq - q).abs() <= q.abs() * 2.0 ** -8 * 1.01 + ref.query_terms(qkv, qn, cos, sin, 1) * 2.0 ** -20).all()
+
+
+@pytest.mark.parametrize("active", [(0, 999), (3, 4, 500, 998), (999,), (0, 1, 2, 700, 701, 997), tuple(range(0, 1000, 37))])
+@pytest.mark.parametrize("hq,hk,hint", [(8, 2, 1), (12, 1, 3), (80, 2, 1)])
+def test_few_active_sequences_among_a_thousand(active, hq, hk, hint):
+    """Slots without rows between those with some, at a run's borders too; their contexts do not matter."""
+    b, rows, ctx = 1000, [0] * 1000, [77] * 1000
+    for j, i in enumerate(active):
+        rows[i], ctx[i] = 1 + j % 3, 5 + 611 * (j % 5) + j
+    num = sum(-(-ctx[i] // 64) for i in active)
+    table = torch.full((b, 41), -1, dtype=torch.int32)
+    at = 0
+    for i in active:
+        n = -(-ctx[i] // 64)
+        table[i, :n] = torch.arange(at, at + n)
+        at += n
+    k, v = _kv(num, hk, 12)
+    pages = ref.pack(k, v)
+    starts, lens = _ints(0, *torch.tensor(rows).cumsum(0).tolist()), _ints(*ctx)
+    q = torch.randn(hq, sum(rows), 128, generator=torch.Generator().manual_seed(6)).to(BF16)
+    got = _run(q, pages, table, starts, lens, 0.1, max_rows=min(hint, sum(rows))).double()
+    want, limit = bounds.attention(q, pages, table, starts, lens, 0.1, registers=min(hint, sum(rows)) * hq // hk <= 32)
+    assert ((got - want).abs() <= limit).all()
