@@ -22,11 +22,11 @@
 //     (S^T = K Q^T, O^T = V^T P^T): with G <= 8 heads a group a tcgen05 tile of 128 rows
 //     would be nearly empty, and its operands would have to be written to shared memory as
 //     bf16, four times the bytes of the codes.  Here a code becomes an operand in a register;
-//   - the instruction issue, above all of the half-rate logic pipe, is what bounds it, so the
-//     nibbles are used where they lie.  Masked with 0x000F / 0x00F0 a pair of them is a pair of
-//     fp16 (K) or bf16 (V) subnormals, u 2^-24 and 16 u 2^-24 or u 2^-133 and 16 u 2^-133
-//     (u = code + 8; eight bits are linear across bf16's first two binades), which the tensor core
-//     multiplies exactly.  Two masks, a shift by 8 and two masks more make eight operands;
+//   - every fragment is a chain of dependent instructions, mostly on the half-rate logic pipe, and an SM
+//     has 16 warps to overlap them, so the nibbles are used where they lie.  Masked with 0x000F / 0x00F0
+//     a pair of them is a pair of fp16 (K) or bf16 (V) subnormals, u 2^-24 and 16 u 2^-24 or u 2^-133 and
+//     16 u 2^-133 (u = code + 8; eight bits are linear across bf16's first two binades), which the tensor
+//     core multiplies exactly.  Two masks, a shift by 8 and two masks more make eight operands;
 //   - K: Q is scaled by a power of two per column into fp16's upper range (its eight bits stay
 //     exact down to 2^-28 of the column's largest value), a sixteenth of it for the channels in
 //     the upper nibbles.  A group's scale multiplies its fp32 sum; what u is too large by,
@@ -42,11 +42,12 @@
 //     a vote finds: p <= 2^8, nothing overflows, and the rescaling is rare.
 // S, the maxima, the sums and O are fp32; P (times V's scale) is rounded to bf16, the type of
 // the tensor core's operand, with relative error 2^-8 of each term.
-// Measured (32 + 8 heads unless said): 64 sequences of 777 to 8192 tokens 89 us, 3.3 TB/s; one of
-// 131001 tokens 48 us, 3.1 TB/s; 16 of 3333 and 4096 tokens, 64 + 8 heads, 31 us, 2.2 TB/s; 16 with a
-// window of 4096 33 us, 2.3 TB/s; one of 321 tokens 8.2 us, latency.  About 350 instructions a
-// fragment of 16 tokens, the half-rate logic pipe some 70% busy in the loop; the copies alone would run
-// at 6 TB/s.
+// Measured (32 + 8 heads unless said): 64 sequences of 777 to 8192 tokens 90 us, 3.3 TB/s; one of
+// 131001 tokens 48.5 us, 3.1 TB/s; 16 of 3333 and 4096 tokens, 64 + 8 heads, 31.5 us, 2.2 TB/s; 16 with a
+// window of 4096 33 us, 2.3 TB/s; one of 321 tokens 8.2 us, latency.  About 350 instructions a fragment of 16
+// tokens.  No pipe is full (issue slots 52%, logic pipe 51% of active cycles): warps wait for their own
+// last instruction, and at the barriers where an item ends (about 5 us a change); the copies alone would
+// run at 6 TB/s.
 #include "kv4.cuh"
 #include "pdl.cuh"
 
@@ -77,8 +78,8 @@ constexpr float UNSEEN = 3e38f;       // 64 - maximum before the first score: fi
 constexpr int MIN_PAGES = GROUPS;     // fewest pages worth a CTA: one a group
 constexpr int ITEM_PAGES = 8;         // what starting and ending an item takes, in pages
 // Items are not cut where the longest has at most so many pages more than an equal run: us apart / cut,
-// 32 + 8 heads, 32 sequences of 256 tokens 10.6 / 17.6, of 2048 tokens 28.1 / 33.6 (5 pages more); 8 of
-// 640 tokens (14 more) 15.0 / 13.3.
+// 32 + 8 heads, in a table of 128 pages: 32 sequences of 256 tokens 11.0 / 17.8, of 2048 tokens 28.3 / 34.1
+// (5 pages more); 8 of 640 tokens (14 more) 13.7 / 13.7.
 constexpr int APART = 10;
 
 // Sequence b's rows, pages and items in the run of pages that the CTAs share: its items, HK for

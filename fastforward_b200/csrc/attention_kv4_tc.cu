@@ -25,11 +25,12 @@
 // A token whose V scale is not finite would poison rows that may not see it (0 x NaN), so its
 // V row is written as zeros and its K row as NaN: exactly the rows that see it become NaN.
 //
-// Measured, 512 rows of each of four sequences over 8704 tokens, 64 + 8 heads: 590 us, 961 TFLOP/s.
+// Measured, 512 rows of each of four sequences over 8704 tokens, 64 + 8 heads: 590 us, 960 TFLOP/s, in short
+// runs; 641 us, 885 TFLOP/s, called over and over (the clocks fall under the power limit).
 // The same walk with the MMAs alone takes 422 us, with the dequantisation 454, with the softmax 540: the
 // MMAs' operands in shared memory bound it first (a block of both tiles reads 192 KB there), then the
 // chain S -> maximum -> exp -> P -> O of a tile, 2400 of a block's 3800 clocks beside 1200 of waiting
-// for S.  64 rows over 2112 tokens, 32 + 8 heads: 22.7 us, of which 5 until the first S and 8 for storing
+// for S.  64 rows over 2112 tokens, 32 + 8 heads: 23 us, of which 5 until the first S and 8 for storing
 // the shares and their join.  Tried and slower: blocks of 64 keys with S held twice (653 us: an MMA
 // of N 64 costs as much as one of 128), four warps for K and four for V (631), a fourth slot for three
 // raw pages (618), a row's scores kept in registers beside four dequantising warps (668), some of

@@ -11,9 +11,10 @@
 // issued together), the last its key and value heads; a row's CTAs are launched next to each
 // other, so that the quantiser's arithmetic runs beside the queries' traffic (behind it: 78 us
 // where this takes 74.6).
-// Measured: 7128 rows of 64 + 8 heads (275 MB) 70.5 us, 3.9 TB/s, of which the queries alone would
-// take 45; the rest is the codes' instructions.  One row of 32 + 8 heads 3.4 us, 320 rows 6.4 us:
-// launch and latency.  Reading those 7128 rows back 11.0 us, 3.4 TB/s.
+// Measured: 7128 rows of 64 + 8 heads (275 MB) 69.9 us, 3.9 TB/s (in four sequences 71.5), of which the
+// queries alone would take 45; 79% of the issue slots are used: the rest is the codes' instructions.  One row
+// of 32 + 8 heads 2.8 us, 320 rows 5.9 us: launch and latency.  Reading those 7128 rows back 10.6 us, 3.5
+// TB/s: a lane has one word of K and one of V on their way.
 //
 // The codes are those of the formula in exact arithmetic, up to fp64's rounding: a key next to
 // the border of two codes must not fall to either side by chance.  Keys are worked out in fp32 with
@@ -264,7 +265,7 @@ __device__ __forceinline__ KeyCodes exact_key(const uint2* x, const uint2* w, co
 }
 
 // Called, it takes no registers of the common path: a fifth CTA an SM for long calls (7128 rows of 64 + 8
-// heads: 74.6 -> 70.5 us).  Where every CTA is resident anyway it is inline (320 rows: 6.9 -> 6.4 us).
+// heads: 4 us of 70).  Where every CTA is resident anyway it is inline (320 rows: 0.5 us of 6).
 __device__ __noinline__ KeyCodes exact_key_call(const uint2* x, const uint2* w, const uint2* c, const uint2* s, float eps,
                                                 int i, uint32_t mask) {
   return exact_key(x, w, c, s, eps, i, mask);
@@ -475,8 +476,9 @@ extern "C" int ffb_qk_norm_rope_kv4(const uint16_t* qkv, int64_t row_stride, con
               "%s: yq and qkv overlap", who);
   WriteArgs a = {qkv, row_stride, q_norm, k_norm, cos, sin, yq, eps, HQ,
                  {pages, page_table, row_start, ctx_len, num_pages, max_pages, B, T, HK, table_stride}};
-  // with few rows every half warp has one head: 320 rows take 10 us so, and 7000 rows a third less
-  // with four
+  // us with one / four query heads a half warp, 64 + 8 heads: 148 rows 4.8 / 5.0, 320 7.2 / 6.3, 592 10.3 / 8.7,
+  // 7128 111 / 70; 16 + 8 heads: 320 rows 5.0 / 5.5, 592 7.1 / 7.4, 2400 19.1 / 19.0, 7128 56 / 50.  The rule
+  // is one for all heads: four from four rows an SM on
   const bool many = T >= 4 * ffb::sm_count();
   const int heads = (many ? 4 : 1) * 2 * WARPS, q_chunks = (HQ + heads - 1) / heads;
   const int rows = T < 65535 ? T : 65535;

@@ -468,8 +468,9 @@ def qk_pair_kv4(qkv, qn, kn, cos, sin, pages, page_table, row_start, ctx_len, ou
     (HQ + 2 HK) * 128] (any row stride that is a multiple of 4, unit last), cos / sin [T, 128]
     (or [1, T, 128]).  Rows [row_start[b], row_start[b + 1]) are the newest tokens of sequence
     b, whose cache holds ctx_len[b] tokens with them, in the pages of page_table[b].  Returns
-    the queries [HQ, T, 128] (`out`, which may be qkv's own memory when T is 1 and must not overlap it
-    otherwise, or a new tensor; rows of no sequence are left as they were).  Norm, rotation and quantisation run in one pass; the queries round once to bf16."""
+    the queries [HQ, T, 128]: `out`, whose rows of no sequence are left as they were (it may be qkv's own
+    memory when T is 1 and must not overlap it otherwise), or a new tensor, whose rows of no sequence are
+    uninitialised.  Norm, rotation and quantisation run in one pass; the queries round once to bf16."""
     place, dev, b, hk = _kv4_place(pages, page_table, row_start, ctx_len)
     qw, kw, eps = qn.weight, kn.weight, qn.variance_epsilon
     if not (qkv.dtype is qw.dtype is kw.dtype is cos.dtype is sin.dtype is BF16):
@@ -498,8 +499,8 @@ def qk_pair_kv4(qkv, qn, kn, cos, sin, pages, page_table, row_start, ctx_len, ou
 
 
 def kv4_read(pages, page_table, row_start, ctx_len, rows):
-    """The newest rows as the 4-bit cache holds them: k, v [HK, rows, 128] bf16, exact.  To read
-    whole sequences, pass row_start with ctx_len's running sums."""
+    """The newest rows as the 4-bit cache holds them: k, v [HK, rows, 128] bf16, exact; rows of no
+    sequence are uninitialised.  To read whole sequences, pass row_start with ctx_len's running sums."""
     if not 0 <= rows <= 1 << 24:
         _need(False, f"rows {rows} (0 to 2^24)")
     place, dev, b, hk = _kv4_place(pages, page_table, row_start, ctx_len)
@@ -516,12 +517,11 @@ def attention_kv4(q, pages, page_table, row_start, ctx_len, scale, window=0, sin
     A row that sees nothing gets zeros.  max_rows: the most rows of one sequence in this call, if
     known (it sizes the launch and changes no result beyond rounding; default T / B, rounded up).  Up to
     32 columns, max_rows HQ / HK, results are held to 2^-79, so that values below about 2^-60 in size lose
-    bits there.
-    Single tokens and long chunks are faster in two calls over the same q and out, each with its
-    slice of row_start, ctx_len and page_table.
-    Held values must be below 2^57 in size.  Returns [T, HQ, 128] bf16 (`out`, which may be q's
-    own memory when T or HQ is 1 and must not overlap it otherwise, or a new tensor; rows of no
-    sequence are left as they were)."""
+    bits there.  Held values must be below 2^57 in size.  Single tokens and long chunks are faster in two
+    calls over the same q and out, each with its slice of row_start, ctx_len and page_table.
+    Returns [T, HQ, 128] bf16: `out`, whose rows of no sequence are left as they were (it may be q's own
+    memory when T or HQ is 1 and must not overlap it otherwise), or a new tensor, whose rows of no sequence
+    are uninitialised."""
     if not (0 <= window <= 1 << 30 and 0 <= sinks <= 1 << 30):  # the C call takes 32 bits of them
         _need(False, f"window {window}, sinks {sinks} (0 to 2^30)")
     place, dev, b, hk = _kv4_place(pages, page_table, row_start, ctx_len)

@@ -476,7 +476,7 @@ int ffb_attention_full(const uint16_t* q, const uint16_t* k, const uint16_t* v, 
  * 2^-100 is held as zeros, one with a value that is not finite or reaches 2^127 as NaN.
  *
  * Every entry takes the same description of its T rows, on the device: row_start [B+1]
- * (ascending): rows [row_start[b], row_start[b+1]) are sequence b's newest tokens (none, one
+ * (ascending, from 0 to T): rows [row_start[b], row_start[b+1]) are sequence b's newest tokens (none, one
  * or many); ctx_len [B]: sequence b's tokens with those rows, so row t has position
  * ctx_len[b] - (row_start[b+1] - t); page_table: B rows of max_pages page ids, table_stride
  * apart; entry i holds positions [64 i, 64 i + 64).  A page may be in several rows of the
