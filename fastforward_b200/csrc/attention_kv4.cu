@@ -677,7 +677,9 @@ __global__ void __launch_bounds__(THREADS, Shape<NT>::PER_SM) kv4_attention_kern
           const bool up = x > high[i];
           const float base = smul[8 * (i >> 1) + 2 * t + (i & 1)];
           float to = 64.f - x * mul[i], to_mul = mul[i], a = ex2(to - neg[i]);
-          if (fabsf(to) > 0x1p30f || to_mul != base) {  // vast scores, or no longer: an old maximum has no weight beside the new
+          // vast scores, or no longer: an old maximum has no weight beside the new one.  What comes out depends on x
+          // alone, so that warps with the same maximum agree
+          if (fabsf(x * mul[i]) >= 0x1p30f || to_mul != base) {
             const float small = vast_scale(x * base);
             to_mul = base * small;
             to = (small == 1.f ? 64.f : 32.f) - x * to_mul;
@@ -1137,8 +1139,8 @@ extern "C" int ffb_attention_kv4(const uint16_t* q, const uint8_t* pages, int nu
     e = kv4::launch_attention_tc(a, (unsigned)p.ctas, st);
     if (e == cudaSuccess && p.cut > 0) e = ffb::launch(kv4_join_tc_kernel, dim3((unsigned)p.cut * 16), dim3(256), 0, st, a);
   } else {
-    // flags and the mark of a failed run (128 bytes, so that rows stay on their lines: off them 131001 tokens take 50.5 us instead of
-    // 48.3), partial rows, their maxima and sums
+    // flags and the mark of a failed run (128 bytes, so that rows stay on their lines: off them 131001 tokens
+    // take 50.5 us instead of 48.3), partial rows, their maxima and sums
     if (!p.splits) {
       a.flags = static_cast<uint64_t*>(ws);
       a.tag = call_tag();

@@ -300,3 +300,24 @@ def test_few_active_sequences_among_a_thousand(active, hq, hk, hint):
     got = _run(q, pages, table, starts, lens, 0.1, max_rows=min(hint, sum(rows))).double()
     want, limit = bounds.attention(q, pages, table, starts, lens, 0.1, registers=min(hint, sum(rows)) * hq // hk <= 32)
     assert ((got - want).abs() <= limit).all()
+
+
+@pytest.mark.parametrize("rows", [1, 4, 40])
+def test_equal_scores_where_they_become_vast(rows):
+    """Two keys of the same score, 2^30 + 48 in base 2, next to which nothing else counts: one is the first that
+    its warps see, one comes after scores of -2^32.  Each has half the weight."""
+    k = torch.full((8, 1, 64, 128), -28.0, dtype=torch.float64)
+    k[1, 0, 3] = k[4, 0, 5] = 7.0
+    _, v = _kv(8, 1, 9)
+    pages = ref.pack(k, v)
+    q = torch.ones(4, rows, 128).to(BF16)
+    near = torch.arange(-64, 64).to(torch.float32) / 16 + 830648.625
+    scale = float(near[(near * torch.tensor(1.4426950408889634)).double() == 1198372.625][0])  # 896 times that: the score
+    table = torch.arange(8, dtype=torch.int32)[None]
+    for width in (8, 100):
+        wide = torch.nn.functional.pad(table, (0, width - 8), value=-1)
+        got = _run(q, pages, wide, _ints(0, rows), _ints(500), scale, max_rows=rows).double()
+        held = ref.unpack(pages)[1][:, 0]
+        want, most = (held[1, 3] + held[4, 5]) / 2, torch.maximum(held[1, 3].abs(), held[4, 5].abs())
+        # a probability's and the result's rounding, and the offsets' 2^-22 255 of a scale
+        assert ((got - want).abs() <= (2 * most + want.abs()) * 2.0 ** -8 * 1.01 + 2.0 ** -14 * most.amax()).all()
